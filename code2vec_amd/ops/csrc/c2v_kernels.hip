@@ -23,24 +23,11 @@
 
 #include <cstdint>
 
-#define DEVI __device__ __forceinline__
-
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
-using u16x8 = __attribute__((ext_vector_type(8))) unsigned short;
-using u16x4 = __attribute__((ext_vector_type(4))) unsigned short;
-using f32x4 = __attribute__((ext_vector_type(4))) float;
-using u32 = uint32_t;
-using u64 = uint64_t;
+#include "c2v_device.h"
 
 // ---------------------------------------------------------------------------
 // small helpers
 // ---------------------------------------------------------------------------
-
-DEVI float bf2f(ushort u) {
-  union { u32 u; float f; } cvt;
-  cvt.u = ((u32)u) << 16;
-  return cvt.f;
-}
 
 DEVI ushort f2bf(float f) {
   // round-to-nearest-even, NaN-safe enough for our ranges
@@ -49,19 +36,6 @@ DEVI ushort f2bf(float f) {
   u32 u = cvt.u;
   u32 rounded = (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
   return (ushort)rounded;
-}
-
-// splitmix64 — must match code2vec_amd/ops/reference.py::_splitmix64 bit-for-bit
-DEVI u64 splitmix64(u64 x) {
-  u64 z = x * 0x9E3779B97F4A7C15ull;
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-  return z ^ (z >> 31);
-}
-
-DEVI float hash_uniform(u64 seed, u64 idx) {
-  u64 h = splitmix64(seed + idx);
-  return (float)((h >> 40) & 0xFFFFFFull) * (1.0f / 16777216.0f);
 }
 
 DEVI float wave_reduce_sum(float v) {
@@ -3420,7 +3394,13 @@ torch::Tensor sampled_ce_bwd(torch::Tensor logits_cand, torch::Tensor labels,
 
 }  // namespace
 
+// defined with their kernels, in files of their own
+void bind_gated(pybind11::module_& mod);
+void bind_mxfp4(pybind11::module_& mod);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
+  bind_gated(mod);
+  bind_mxfp4(mod);
   mod.def("gather_concat_fwd", &gather_concat_fwd);
   mod.def("gather_concat_bwd", &gather_concat_bwd);
   mod.def("transform_tanh_fwd", &transform_tanh_fwd);

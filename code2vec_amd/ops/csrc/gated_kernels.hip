@@ -1,0 +1,642 @@
+// The gated context transform (gfx950), forward and backward.
+//
+//   g = x Wg^T,  u = x Wu^T,  y = act(g) * u                     x (N,K)
+//   du = dy * act(g),  dg = dy * u * act'(g)
+//   dx = dg Wg + du Wu,  dW = x^T [dg | du]
+//
+// bf16 operands, fp32 accumulation and fp32 activations. What is rounded to
+// bf16 on the way: g and u as they are kept for the backward, and dg and du
+// as operands of the two products that consume them; each such value enters
+// sums of 2H or N terms, so that a rounding of 2^-9 of a term stays one of
+// about 2^-9 of the result, which is itself rounded to bf16.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+
+#include "c2v_device.h"
+
+namespace {
+
+enum Activation : int { SILU = 0, GELU = 1, SIGMOID = 2, TANH = 3, RELU = 4 };
+
+template <int ACT>
+DEVI float act_fwd(float g) {
+  if constexpr (ACT == SILU) return g / (1.f + __expf(-g));
+  if constexpr (ACT == GELU) return 0.5f * g * (1.f + erff(g * 0.70710678f));
+  if constexpr (ACT == SIGMOID) return 1.f / (1.f + __expf(-g));
+  if constexpr (ACT == TANH) return tanhf(g);
+  return g > 0.f ? g : (g != g ? g : 0.f);
+}
+
+// act(g) and act'(g)
+template <int ACT>
+DEVI void act_both(float g, float& a, float& da) {
+  if constexpr (ACT == SILU) {
+    const float s = 1.f / (1.f + __expf(-g));
+    a = g * s;
+    da = s * (1.f + g * (1.f - s));
+  } else if constexpr (ACT == GELU) {
+    const float cdf = 0.5f * (1.f + erff(g * 0.70710678f));
+    a = g * cdf;
+    da = cdf + g * __expf(-0.5f * g * g) * 0.39894228f;
+  } else if constexpr (ACT == SIGMOID) {
+    a = 1.f / (1.f + __expf(-g));
+    da = a * (1.f - a);
+  } else if constexpr (ACT == TANH) {
+    a = tanhf(g);
+    da = 1.f - a * a;
+  } else {
+    a = g > 0.f ? g : (g != g ? g : 0.f);
+    da = g > 0.f ? 1.f : 0.f;
+  }
+}
+
+DEVI void to_lds16(const ushort* src, ushort* dst) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) u32*)src,
+      (__attribute__((address_space(3))) u32*)dst, 16, 0, 0);
+}
+
+// what a chunk beyond the reduction's end reads
+__device__ __attribute__((aligned(16))) const ushort k_zero_chunk[8] = {};
+
+DEVI u16x8 pack8(const float* v) {
+  bf16x8 b;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = (__bf16)v[j];
+  return __builtin_bit_cast(u16x8, b);
+}
+
+// ---------------------------------------------------------------------------
+// Products whose reduction runs along the rows of both operands.
+//
+// The weights take the place of the matrix instruction's A operand and the
+// rows of x that of its B operand: a lane then holds consecutive output
+// columns of ONE row. Weight rows are put into LDS in such an order that the
+// 4 x GT values of a lane in one group of GT tiles are 4*GT consecutive
+// columns, which go out as 16-byte stores. A wave has two groups: the gate
+// and the up columns of the same outputs, or two neighbours for a plain
+// product.
+// ---------------------------------------------------------------------------
+
+constexpr int BK = 64;   // reduction values a step: rows of 128 bytes in LDS
+
+enum Epilogue : int { GATED = 0, PLAIN = 1 };
+
+struct BtArgs {
+  const ushort* x;    // (N, K), rows ldx apart
+  const ushort* w;    // GATED: (2, H, K); PLAIN: (H, K)
+  ushort* y;          // (N, H)
+  ushort* gu;         // GATED: (N, 2, Hp) or null
+  long ldx;
+  int N, H, Hp, K;
+  float keep_prob;    // PLAIN with dropout: below one
+  u64 seed;
+  const long* seed_ptr;
+};
+
+template <int EPI, int ACT, int WR, int WC, int XT, int GT>
+__launch_bounds__(WR * WC * 64)
+__global__ void k_rows_gemm(BtArgs p) {
+  constexpr int T = WR * WC * 64;
+  constexpr int BM = WR * XT * 16;         // rows of x a block
+  constexpr int BG = WC * GT * 16;         // columns of one group
+  constexpr int BN = 2 * BG;               // rows of w a block
+  constexpr int HT = EPI == GATED ? BG : BN;   // output columns a block
+  constexpr int CH = BK / 8;               // 16-byte chunks a row
+  constexpr int IT = (BM + BN) * CH / T;
+  static_assert((BM + BN) * CH % T == 0 && BM * CH % 64 == 0, "staging");
+  extern __shared__ ushort lds[];          // 2 x (BM + BN) x BK
+
+  const int nC = (p.H + HT - 1) / HT;
+  const int wg = xcd_chunked(blockIdx.x, gridDim.x);
+  const long row0 = (long)(wg / nC) * BM;
+  const int h0 = (wg % nC) * HT;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wid / WC, wc = wid % WC;
+  const int l16 = lane & 15, q = lane >> 4;
+
+  // this thread's source rows, one for each chunk that it stages
+  const ushort* src[IT];
+  int col[IT];
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int c = it * T + tid;
+    const int r = c / CH, pos = c % CH;
+    col[it] = (pos ^ (r & 7)) * 8;
+    if (r < BM) {
+      const long n = min(row0 + r, (long)p.N - 1);
+      src[it] = p.x + n * p.ldx;
+    } else {
+      const int j = r - BM;                       // row of w in LDS
+      const int i = j & 15, mi = (j >> 4) % GT;
+      const int grp = (j >> 4) / GT % 2, cw = (j >> 4) / (2 * GT);
+      const int in_group = (i >> 2) * (4 * GT) + mi * 4 + (i & 3);
+      long wrow;
+      if constexpr (EPI == GATED)
+        wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
+      else
+        wrow = min(h0 + (cw * 2 + grp) * GT * 16 + in_group, p.H - 1);
+      src[it] = p.w + wrow * p.K;
+    }
+  }
+  auto stage = [&](int k0, int buf) {
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      const int k = k0 + col[it];
+      const ushort* s = k < p.K ? src[it] + k : k_zero_chunk;
+      to_lds16(s, lds + (long)buf * (BM + BN) * BK + (it * T + wid * 64) * 8);
+    }
+  };
+
+  f32x4 acc[XT][2 * GT];
+#pragma unroll
+  for (int i = 0; i < XT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2 * GT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+
+  const int steps = (p.K + BK - 1) / BK;
+  stage(0, 0);
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    if (s + 1 < steps) stage((s + 1) * BK, (s + 1) & 1);
+    const ushort* xs = lds + (s & 1) * (BM + BN) * BK + wr * XT * 16 * BK;
+    const ushort* ws = lds + (s & 1) * (BM + BN) * BK +
+                       (BM + wc * 2 * GT * 16) * BK;
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      const int off = l16 * BK + (((kk * 4 + q) ^ (l16 & 7)) * 8);
+      bf16x8 xf[XT], wf[2 * GT];
+#pragma unroll
+      for (int i = 0; i < XT; ++i)
+        xf[i] = *reinterpret_cast<const bf16x8*>(xs + i * 16 * BK + off);
+#pragma unroll
+      for (int j = 0; j < 2 * GT; ++j)
+        wf[j] = *reinterpret_cast<const bf16x8*>(ws + j * 16 * BK + off);
+#pragma unroll
+      for (int i = 0; i < XT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2 * GT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              wf[j], xf[i], acc[i][j], 0, 0, 0);
+    }
+    __syncthreads();
+  }
+
+  const bool vec = (p.H & 7) == 0;
+  const u64 seed = p.seed_ptr ? (u64)*p.seed_ptr : p.seed;
+  const float inv_keep = 1.f / p.keep_prob;
+  // run = values of one lane in one group, consecutive columns from h
+  auto put = [&](ushort* base, const float* v, int h) {
+#pragma unroll
+    for (int c = 0; c < 4 * GT; c += 4) {
+      if (vec && GT >= 2) {
+        if (c % 8 == 0 && h + c < p.H)
+          *reinterpret_cast<u16x8*>(base + c) = pack8(v + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (h + c + j < p.H)
+            base[c + j] = __builtin_bit_cast(ushort, (__bf16)v[c + j]);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < XT; ++i) {
+    const long n = row0 + wr * XT * 16 + i * 16 + l16;
+    if (n >= p.N) continue;
+    if constexpr (EPI == GATED) {
+      const int h = h0 + wc * GT * 16 + q * 4 * GT;
+      float gv[4 * GT], uv[4 * GT], yv[4 * GT];
+#pragma unroll
+      for (int j = 0; j < GT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          gv[j * 4 + r] = acc[i][j][r];
+          uv[j * 4 + r] = acc[i][GT + j][r];
+          yv[j * 4 + r] = act_fwd<ACT>(acc[i][j][r]) * acc[i][GT + j][r];
+        }
+      put(p.y + n * p.H + h, yv, h);
+      if (p.gu) {
+        put(p.gu + n * 2 * p.Hp + h, gv, h);
+        put(p.gu + n * 2 * p.Hp + p.Hp + h, uv, h);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int h = h0 + (wc * 2 + g) * GT * 16 + q * 4 * GT;
+        float v[4 * GT];
+#pragma unroll
+        for (int j = 0; j < GT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float t = acc[i][g * GT + j][r];
+            if (p.keep_prob < 1.f) {
+              const u64 e = (u64)n * p.H + h + j * 4 + r;
+              t = hash_uniform(seed, e) < p.keep_prob ? t * inv_keep : 0.f;
+            }
+            v[j * 4 + r] = t;
+          }
+        put(p.y + n * p.H + h, v, h);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dg and du from what the forward kept. One pass: reads gu and dy, writes
+// dgu; bound by memory. Columns H..Hp of each half are written as zeros, so
+// that the products below run over whole chunks.
+// ---------------------------------------------------------------------------
+
+template <int ACT>
+__launch_bounds__(256)
+__global__ void k_gated_dgu(const ushort* __restrict__ gu,
+                            const ushort* __restrict__ dy, long lddy,
+                            ushort* __restrict__ dgu, long N, int H, int Hp,
+                            int vec) {
+  const int per_row = Hp / 8;
+  const long total = N * per_row;
+  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < total;
+       c += (long)gridDim.x * 256) {
+    const long n = c / per_row;
+    const int h = (int)(c % per_row) * 8;
+    const ushort* gp = gu + n * 2 * Hp + h;
+    const u16x8 g8 = *reinterpret_cast<const u16x8*>(gp);
+    const u16x8 u8 = *reinterpret_cast<const u16x8*>(gp + Hp);
+    const ushort* dp = dy + n * lddy + h;
+    u16x8 d8 = {};
+    if (vec) {
+      d8 = *reinterpret_cast<const u16x8*>(dp);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (h + j < H) d8[j] = dp[j];
+    }
+    float dg[8], du[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float a, da;
+      act_both<ACT>(bf2f(g8[j]), a, da);
+      const float d = bf2f(d8[j]);
+      dg[j] = h + j < H ? d * bf2f(u8[j]) * da : 0.f;
+      du[j] = h + j < H ? d * a : 0.f;
+    }
+    ushort* op = dgu + n * 2 * Hp + h;
+    *reinterpret_cast<u16x8*>(op) = pack8(dg);
+    *reinterpret_cast<u16x8*>(op + Hp) = pack8(du);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dW: the reduction runs down the columns of both operands, over N rows. The
+// tiles lie in LDS as they lie in memory, and the transposing LDS read hands
+// each lane four rows of its column. The order of the rows within a step of
+// 32 is the same for both operands and does not matter to the sum: lane
+// group q takes rows 4q..4q+3 and 16+4q..16+4q+3, so that one read covers 16
+// neighbouring rows, whose 32-byte units the exclusive-or below spreads over
+// all banks. N is split over gridDim.y; the parts are added in order by
+// k_dw_reduce, so that a result never depends on timing.
+// ---------------------------------------------------------------------------
+
+constexpr int TN_ROWS = 32;
+
+DEVI bf16x8 tr_read(const ushort* tile, int stride, int c0, int l16, int q) {
+  s16x4 v[2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = half * 16 + q * 4 + (l16 >> 2);
+    const int unit = (c0 >> 4) ^ (r & 7);
+    const ushort* a = tile + r * stride + unit * 16 + (l16 & 3) * 4;
+    v[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)a);
+  }
+  bf16x4 lo = __builtin_bit_cast(bf16x4, v[0]);
+  bf16x4 hi = __builtin_bit_cast(bf16x4, v[1]);
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <int WA, int WB, int AT, int BT>
+__launch_bounds__(WA * WB * 64)
+__global__ void k_dw_part(const ushort* __restrict__ dgu,
+                          const ushort* __restrict__ x, long ldx,
+                          float* __restrict__ part, int N, int C2, int K,
+                          int K8, int rows_each) {
+  constexpr int T = WA * WB * 64;
+  constexpr int CA = WA * AT * 16;     // columns of dgu a block
+  constexpr int CB = WB * BT * 16;     // columns of x a block
+  constexpr int ITA = TN_ROWS * CA / 8 / T, ITB = TN_ROWS * CB / 8 / T;
+  static_assert(TN_ROWS * CA / 8 % T == 0 && TN_ROWS * CB / 8 % T == 0, "staging");
+  extern __shared__ ushort lds[];
+  constexpr int BUF = TN_ROWS * (CA + CB);
+
+  const int nB = (K + CB - 1) / CB;
+  const int a0 = blockIdx.x / nB * CA, b0 = blockIdx.x % nB * CB;
+  const long n0 = (long)blockIdx.y * rows_each;
+  const long n1 = min(n0 + rows_each, (long)N);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wa = wid / WB, wb = wid % WB;
+  const int l16 = lane & 15, q = lane >> 4;
+
+  auto stage = [&](long n, int buf) {
+    ushort* la = lds + buf * BUF;
+    ushort* lb = la + TN_ROWS * CA;
+#pragma unroll
+    for (int it = 0; it < ITA; ++it) {
+      const int c = it * T + tid;
+      const int r = c / (CA / 8), pos = c % (CA / 8);
+      const int cc = a0 + (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
+      const ushort* s = (n + r < n1 && cc < C2) ? dgu + (n + r) * C2 + cc
+                                                : k_zero_chunk;
+      to_lds16(s, la + (it * T + wid * 64) * 8);
+    }
+#pragma unroll
+    for (int it = 0; it < ITB; ++it) {
+      const int c = it * T + tid;
+      const int r = c / (CB / 8), pos = c % (CB / 8);
+      const int cc = b0 + (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
+      const ushort* s = (n + r < n1 && cc < K8) ? x + (n + r) * ldx + cc
+                                                : k_zero_chunk;
+      to_lds16(s, lb + (it * T + wid * 64) * 8);
+    }
+  };
+
+  f32x4 acc[AT][BT];
+#pragma unroll
+  for (int i = 0; i < AT; ++i)
+#pragma unroll
+    for (int j = 0; j < BT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+
+  const int steps = (int)((n1 - n0 + TN_ROWS - 1) / TN_ROWS);
+  if (steps > 0) stage(n0, 0);
+  __syncthreads();
+  for (int s = 0; s < steps; ++s) {
+    if (s + 1 < steps) stage(n0 + (long)(s + 1) * TN_ROWS, (s + 1) & 1);
+    const ushort* la = lds + (s & 1) * BUF;
+    const ushort* lb = la + TN_ROWS * CA;
+    bf16x8 af[AT], bf[BT];
+#pragma unroll
+    for (int i = 0; i < AT; ++i)
+      af[i] = tr_read(la, CA, (wa * AT + i) * 16, l16, q);
+#pragma unroll
+    for (int j = 0; j < BT; ++j)
+      bf[j] = tr_read(lb, CB, (wb * BT + j) * 16, l16, q);
+#pragma unroll
+    for (int i = 0; i < AT; ++i)
+#pragma unroll
+      for (int j = 0; j < BT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[i], bf[j],
+                                                            acc[i][j], 0, 0, 0);
+    __syncthreads();
+  }
+  // part (S, K, C2): a lane holds four consecutive columns of C2
+#pragma unroll
+  for (int j = 0; j < BT; ++j) {
+    const int k = b0 + (wb * BT + j) * 16 + l16;
+    if (k >= K) continue;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      const int c = a0 + (wa * AT + i) * 16 + q * 4;
+      if (c < C2)
+        *reinterpret_cast<f32x4*>(part + ((long)blockIdx.y * K + k) * C2 + c) =
+            acc[i][j];
+    }
+  }
+}
+
+// d_w (2, K, H) bf16 from the parts (S, K, 2, Hp)
+__launch_bounds__(256)
+__global__ void k_dw_reduce(const float* __restrict__ part,
+                            ushort* __restrict__ d_w, int S, int K, int H,
+                            int Hp) {
+  const long quads = (long)K * 2 * Hp / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= quads) return;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < S; ++s)
+    sum += *reinterpret_cast<const f32x4*>(part + (s * quads + i) * 4);
+  const long k = i * 4 / (2 * Hp);
+  const int c = (int)(i * 4 % (2 * Hp));
+  const int g = c / Hp, h = c % Hp;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (h + j < H)
+      d_w[((long)g * K + k) * H + h + j] =
+          __builtin_bit_cast(ushort, (__bf16)sum[j]);
+}
+
+// (R, C) with rows ld apart -> (R, Cp), the columns behind C zero
+__launch_bounds__(256)
+__global__ void k_pad_cols(const ushort* __restrict__ in, long ld,
+                           ushort* __restrict__ out, long R, int C, int Cp) {
+  const long total = R * (Cp / 8);
+  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < total;
+       c += (long)gridDim.x * 256) {
+    const long r = c / (Cp / 8);
+    const int k = (int)(c % (Cp / 8)) * 8;
+    u16x8 v = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < C) v[j] = in[r * ld + k + j];
+    *reinterpret_cast<u16x8*>(out + r * Cp + k) = v;
+  }
+}
+
+// ===========================================================================
+// host wrappers
+// ===========================================================================
+
+inline hipStream_t cur_stream() {
+  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+}
+
+inline int pad8(int v) { return (v + 7) / 8 * 8; }
+
+inline int grid_of(long items, int block, long cap) {
+  return (int)std::max(1L, std::min((items + block - 1) / block, cap));
+}
+
+const ushort* bf_ptr(const torch::Tensor& t) {
+  return reinterpret_cast<const ushort*>(t.data_ptr<at::BFloat16>());
+}
+ushort* bf_mut(const torch::Tensor& t) {
+  return reinterpret_cast<ushort*>(t.data_ptr<at::BFloat16>());
+}
+
+void check_bf16(const torch::Tensor& t, const char* name, int dims,
+                const torch::Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on the GPU that ctx is on");
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be bfloat16");
+  TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " dimensions");
+}
+
+// Rows whose values follow each other, start on 16 bytes and are a multiple
+// of eight long: `t` itself, or a padded copy of it.
+struct Rows {
+  torch::Tensor held;
+  const ushort* p;
+  long ld;
+};
+
+Rows chunked_rows(const torch::Tensor& t, int cols) {
+  const bool dense = t.size(1) <= 1 || t.stride(1) == 1;
+  const long ld = t.size(0) <= 1 ? pad8(cols) : t.stride(0);
+  if (dense && cols % 8 == 0 && ld % 8 == 0 && ld >= 0 &&
+      (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0)
+    return {t, bf_ptr(t), ld};
+  auto src = dense ? t : t.contiguous();
+  auto out = torch::empty({t.size(0), (long)pad8(cols)}, t.options());
+  const long items = t.size(0) * (pad8(cols) / 8);
+  k_pad_cols<<<grid_of(items, 256, 8192), 256, 0, cur_stream()>>>(
+      bf_ptr(src), src.size(0) <= 1 ? cols : src.stride(0), bf_mut(out),
+      t.size(0), cols, pad8(cols));
+  return {out, bf_ptr(out), (long)pad8(cols)};
+}
+
+template <int EPI, int ACT, int WR, int WC, int XT, int GT>
+void launch_rows(const BtArgs& a) {
+  constexpr int BM = WR * XT * 16, BG = WC * GT * 16;
+  constexpr int HT = EPI == GATED ? BG : 2 * BG;
+  constexpr size_t bytes = 2ul * (BM + 2 * BG) * BK * sizeof(ushort);
+  auto* fn = &k_rows_gemm<EPI, ACT, WR, WC, XT, GT>;
+  if (bytes > 64 * 1024)
+    C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
+                                       hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)bytes));
+  const long tiles = ((long)a.N + BM - 1) / BM * ((a.H + HT - 1) / HT);
+  TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
+  fn<<<(int)tiles, WR * WC * 64, bytes, cur_stream()>>>(a);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+template <int EPI, int ACT>
+void rows_gemm(const BtArgs& a) {
+  launch_rows<EPI, ACT, 4, 2, 4, 4>(a);
+}
+
+template <int ACT>
+void launch_dgu(const ushort* gu, const ushort* dy, long lddy, ushort* dgu,
+                long N, int H, int Hp, int vec) {
+  auto* fn = &k_gated_dgu<ACT>;
+  fn<<<grid_of(N * (Hp / 8), 256, 8192), 256, 0, cur_stream()>>>(
+      gu, dy, lddy, dgu, N, H, Hp, vec);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+}
+
+#define WITH_ACT(act, ...)                                              \
+  switch (act) {                                                        \
+    case SILU: { constexpr int A = SILU; __VA_ARGS__; break; }          \
+    case GELU: { constexpr int A = GELU; __VA_ARGS__; break; }          \
+    case SIGMOID: { constexpr int A = SIGMOID; __VA_ARGS__; break; }    \
+    case TANH: { constexpr int A = TANH; __VA_ARGS__; break; }          \
+    case RELU: { constexpr int A = RELU; __VA_ARGS__; break; }          \
+    default: TORCH_CHECK(false, "unknown activation ", act);            \
+  }
+
+// y (N,H), and gu (N,2,Hp) when it is kept (empty otherwise)
+std::vector<torch::Tensor> transform_gated_fwd(torch::Tensor ctx,
+                                               torch::Tensor w_oi, int64_t act,
+                                               bool save) {
+  check_bf16(ctx, "ctx", 2, ctx);
+  check_bf16(w_oi, "w_oi", 3, ctx);
+  TORCH_CHECK(w_oi.size(0) == 2 && w_oi.size(2) == ctx.size(1) &&
+              w_oi.is_contiguous(), "w_oi must be a contiguous (2, H, K)");
+  TORCH_CHECK(ctx.size(0) < (1L << 31) && ctx.size(1) < (1L << 24) &&
+              w_oi.size(1) < (1L << 24), "ctx or w_oi is too large");
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
+  const int N = ctx.size(0), K = ctx.size(1), H = w_oi.size(1), Hp = pad8(H);
+  auto y = torch::empty({N, H}, ctx.options());
+  auto gu = torch::empty({save ? N : 0, 2, Hp}, ctx.options());
+  if (N == 0 || H == 0) return {y, gu};
+  const Rows x = chunked_rows(ctx, K), w = chunked_rows(w_oi.view({2L * H, K}), K);
+  BtArgs a{x.p, w.p, bf_mut(y), save ? bf_mut(gu) : nullptr, x.ld, N, H, Hp,
+           pad8(K), 1.f, 0, nullptr};
+  WITH_ACT(act, (rows_gemm<GATED, A>(a)));
+  return {y, gu};
+}
+
+// d_ctx (N,K) and d_w (2,K,H)
+std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
+                                               torch::Tensor w_io,
+                                               torch::Tensor gu,
+                                               torch::Tensor d_y, int64_t act,
+                                               double keep_prob, int64_t seed,
+                                               torch::Tensor seed_t) {
+  check_bf16(ctx, "ctx", 2, ctx);
+  check_bf16(w_io, "w_io", 2, ctx);
+  check_bf16(gu, "gu", 3, ctx);
+  check_bf16(d_y, "d_y", 2, ctx);
+  const int N = ctx.size(0), K = ctx.size(1), H = d_y.size(1), Hp = pad8(H);
+  TORCH_CHECK(d_y.size(0) == N, "d_y must have as many rows as ctx");
+  TORCH_CHECK(w_io.size(0) == K && w_io.size(1) == 2L * H && w_io.is_contiguous(),
+              "w_io must be a contiguous (K, 2H)");
+  TORCH_CHECK(gu.size(0) == N && gu.size(1) == 2 && gu.size(2) == Hp &&
+              gu.is_contiguous(), "gu must be what the forward kept");
+  TORCH_CHECK(keep_prob > 0.0 && keep_prob <= 1.0, "keep_prob must be in (0, 1]");
+  const long* seed_ptr = nullptr;
+  if (seed_t.defined() && seed_t.numel() == 1) {
+    TORCH_CHECK(seed_t.device() == ctx.device() &&
+                seed_t.scalar_type() == torch::kInt64,
+                "seed_t must be one int64 on the GPU that ctx is on");
+    seed_ptr = seed_t.data_ptr<long>();
+  }
+  const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
+  auto d_ctx = torch::empty({N, K}, ctx.options());
+  if (N == 0 || H == 0 || K == 0)
+    return {d_ctx.zero_(), torch::zeros({2, K, H}, ctx.options())};
+
+  auto dgu = torch::empty_like(gu);
+  {
+    const bool dense = H == 1 || d_y.stride(1) == 1;
+    auto dy = dense ? d_y : d_y.contiguous();
+    const long lddy = N == 1 ? H : dy.stride(0);
+    const int vec = H % 8 == 0 && lddy % 8 == 0 &&
+                    (reinterpret_cast<uintptr_t>(dy.data_ptr()) & 15) == 0;
+    WITH_ACT(act, launch_dgu<A>(bf_ptr(gu), bf_ptr(dy), lddy, bf_mut(dgu), N, H,
+                                Hp, vec));
+  }
+
+  Rows w;
+  if (H == Hp) {
+    w = chunked_rows(w_io, 2 * H);
+  } else {
+    w = chunked_rows(w_io.view({2L * K, H}), H);   // (K, 2, Hp)
+  }
+  BtArgs a{bf_ptr(dgu), w.p, bf_mut(d_ctx), nullptr, 2L * Hp, N, K, pad8(K),
+           2 * Hp, (float)keep_prob, (u64)seed, seed_ptr};
+  rows_gemm<PLAIN, SILU>(a);
+
+  const Rows x = chunked_rows(ctx, K);
+  constexpr int WA = 2, WB = 2, AT = 8, BT = 4;
+  const int tiles = (2 * Hp + WA * AT * 16 - 1) / (WA * AT * 16) *
+                    ((K + WB * BT * 16 - 1) / (WB * BT * 16));
+  const long most = ((long)N + 255) / 256;   // at least 256 rows a part
+  const int S = (int)std::max(1L, std::min(most, (long)(512 + tiles - 1) / tiles));
+  const int rows_each = (int)((((long)N + S - 1) / S + TN_ROWS - 1) / TN_ROWS * TN_ROWS);
+  auto part = torch::empty({S, K, 2L * Hp}, ctx.options().dtype(torch::kFloat32));
+  constexpr size_t bytes = 2ul * TN_ROWS * (WA * AT + WB * BT) * 16 * sizeof(ushort);
+  auto* dw = &k_dw_part<WA, WB, AT, BT>;
+  dw<<<dim3(tiles, S), WA * WB * 64, bytes, cur_stream()>>>(
+      bf_ptr(dgu), x.p, x.ld, part.data_ptr<float>(), N, 2 * Hp, K, pad8(K),
+      rows_each);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  auto d_w = torch::empty({2, K, H}, ctx.options());
+  const long quads = (long)K * 2 * Hp / 4;
+  k_dw_reduce<<<(int)((quads + 255) / 256), 256, 0, cur_stream()>>>(
+      part.data_ptr<float>(), bf_mut(d_w), S, K, H, Hp);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  return {d_ctx, d_w};
+}
+
+}  // namespace
+
+void bind_gated(pybind11::module_& mod) {
+  mod.def("transform_gated_fwd", &transform_gated_fwd);
+  mod.def("transform_gated_bwd", &transform_gated_bwd);
+}

@@ -3,12 +3,13 @@ the pure-torch reference on CPU. The HIP path is mandatory on GPU (see
 ops/__init__.backend_for) — no silent eager fallback."""
 
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
 from . import backend_for, hip_ext
 from . import reference as ref
+from .reference import GATE_ACTIVATIONS, Mxfp4
 
 
 def gather_concat_fwd(tok_table, path_table, src_ids, path_ids, tgt_ids,
@@ -62,6 +63,140 @@ def transform_tanh_bwd(ctx, w_io_bf16, y, d_y) -> Tuple[torch.Tensor, torch.Tens
     d_ctx = d_zr @ w_io_bf16.to(d_zr.dtype).t()
     d_w = (ctx.t().float() @ d_zr.float())
     return d_ctx, d_w
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise ValueError(what)
+
+
+def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
+                        ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gated transform: y = act(ctx Wg^T) * (ctx Wu^T), both projections, the
+    activation and the product in one kernel.
+
+    ctx (N,K); w_oi (2,H,K), gate then up, out-major like the tanh
+    transform's shadow; activation one of GATE_ACTIVATIONS. Returns (y (N,H),
+    gu): gu holds what transform_gated_bwd needs if `save`, else None. On the
+    GPU all are bfloat16 (sums and activation in fp32), any N, K and H; rows
+    of ctx may be any stride apart."""
+    _need(activation in GATE_ACTIVATIONS, 'activation must be one of %s, not %r'
+          % (', '.join(GATE_ACTIVATIONS), activation))
+    _need(ctx.dim() == 2 and w_oi.dim() == 3 and w_oi.shape[0] == 2
+          and w_oi.shape[2] == ctx.shape[1],
+          'ctx (N,K) and w_oi (2,H,K) do not fit: %s and %s'
+          % (tuple(ctx.shape), tuple(w_oi.shape)))
+    _need(ctx.dtype == w_oi.dtype and ctx.device == w_oi.device,
+          'ctx and w_oi must have one type and one device')
+    if backend_for(ctx) == 'hip':
+        y, gu = hip_ext(True).transform_gated_fwd(
+            ctx, w_oi, GATE_ACTIVATIONS.index(activation), bool(save))
+        return y, gu if save else None
+    return ref.transform_gated_fwd(ctx, w_oi, activation, save)
+
+
+def transform_gated_bwd(ctx, w_io, gu, d_y, activation: str = 'silu',
+                        keep_prob: float = 1.0, seed: int = 0, seed_t=None
+                        ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Backward of the gated transform. ctx as in the forward; w_io (K,2H)
+    the same weights in-major, gate columns then up columns; gu what the
+    forward kept; d_y (N,H). Returns (d_ctx (N,K), d_w (2,K,H)), in ctx's
+    type. With keep_prob < 1 d_ctx goes through the keep mask of the dropout
+    that made ctx (gather_concat_fwd with the same seed) on its way out."""
+    _need(activation in GATE_ACTIVATIONS, 'activation must be one of %s, not %r'
+          % (', '.join(GATE_ACTIVATIONS), activation))
+    _need(ctx.dim() == 2 and d_y.dim() == 2 and d_y.shape[0] == ctx.shape[0]
+          and tuple(w_io.shape) == (ctx.shape[1], 2 * d_y.shape[1]),
+          'ctx (N,K), w_io (K,2H) and d_y (N,H) do not fit: %s, %s and %s'
+          % (tuple(ctx.shape), tuple(w_io.shape), tuple(d_y.shape)))
+    _need(gu is not None, 'the forward kept nothing: call it with save=True')
+    _need(tuple(gu.shape) == (ctx.shape[0], 2, -(-d_y.shape[1] // 8) * 8),
+          'gu is not what the forward of this ctx kept')
+    _need(all(t.dtype == ctx.dtype and t.device == ctx.device
+              for t in (w_io, gu, d_y)),
+          'ctx, w_io, gu and d_y must have one type and one device')
+    _need(0.0 < keep_prob <= 1.0, 'keep_prob must be in (0, 1]')
+    if backend_for(ctx) == 'hip':
+        d_ctx, d_w = hip_ext(True).transform_gated_bwd(
+            ctx, w_io, gu, d_y, GATE_ACTIVATIONS.index(activation),
+            float(keep_prob), int(seed),
+            seed_t if seed_t is not None else torch.empty(0))
+        return d_ctx, d_w
+    d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, gu, d_y, activation)
+    if keep_prob < 1.0:
+        if seed_t is not None:
+            seed = int(seed_t.item())
+        d_ctx = ref.gather_concat_bwd(d_ctx, keep_prob, seed, True)
+    return d_ctx, d_w
+
+
+def _check_mxfp4(q, name: str):
+    _need(isinstance(q, Mxfp4), '%s must be an Mxfp4' % name)
+    blocks = -(-q.k // ref.MXFP4_BLOCK)
+    _need(q.codes.dtype == torch.uint8 and q.scales.dtype == torch.uint8,
+          '%s must hold uint8 codes and scales' % name)
+    _need(q.codes.dim() == 2 and q.scales.dim() == 2
+          and q.codes.shape[0] == q.scales.shape[0]
+          and q.scales.shape[1] == blocks and q.codes.shape[1] == 16 * blocks,
+          '%s does not hold rows of %d values: codes %s, scales %s'
+          % (name, q.k, tuple(q.codes.shape), tuple(q.scales.shape)))
+    _need(q.codes.is_contiguous() and q.scales.is_contiguous()
+          and q.codes.device == q.scales.device,
+          '%s must be contiguous and on one device' % name)
+
+
+def mxfp4_quantize(x) -> Mxfp4:
+    """Rows x (N,K), float32 or bfloat16, to MXFP4: blocks of 32 values along
+    a row under one power of two, each value a 4-bit float (e2m1), rounded to
+    nearest even and saturating. A block that holds a NaN or an infinity
+    becomes NaN. Any N and K, rows any stride apart."""
+    _need(x.dim() == 2, 'x must be (N,K), not %s' % (tuple(x.shape),))
+    _need(x.dtype in (torch.float32, torch.bfloat16),
+          'x must be float32 or bfloat16, not %s' % x.dtype)
+    if backend_for(x) == 'hip':
+        codes, scales = hip_ext(True).mxfp4_quantize(x)
+        return Mxfp4(codes, scales, x.shape[1])
+    return ref.mxfp4_quantize(x)
+
+
+def mxfp4_dequantize(q: Mxfp4, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values that q stands for, (N,K). They are exact in either dtype,
+    bfloat16 or float32."""
+    _check_mxfp4(q, 'q')
+    _need(dtype in (torch.float32, torch.bfloat16),
+          'dtype must be float32 or bfloat16, not %s' % dtype)
+    if backend_for(q.codes) == 'hip':
+        return hip_ext(True).mxfp4_dequantize(q.codes, q.scales, q.k,
+                                              dtype == torch.float32)
+    return ref.mxfp4_dequantize(q, dtype)
+
+
+def mxfp4_matmul(x, w: Mxfp4, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """x (N,K) times the transpose of w (M,K): (N,M) in out_dtype, bfloat16
+    or float32, summed in fp32.
+
+    x a bfloat16 tensor: only the weights are in 4 bits, decoded on the way
+    into the matrix instructions, which is exact. x an Mxfp4: both sides go
+    into the scaled matrix instructions as they are. Any N, M and K. There is
+    no backward: this is what a trained table answers with."""
+    _check_mxfp4(w, 'w')
+    _need(out_dtype in (torch.float32, torch.bfloat16),
+          'out_dtype must be float32 or bfloat16, not %s' % out_dtype)
+    if isinstance(x, Mxfp4):
+        _check_mxfp4(x, 'x')
+        _need(x.k == w.k, 'x has rows of %d values, w of %d' % (x.k, w.k))
+        _need(x.codes.device == w.codes.device, 'x and w must be on one device')
+        if backend_for(w.codes) == 'hip':
+            return hip_ext(True).mxfp4_matmul(x.codes, x.scales, w.codes, w.scales,
+                                              w.k, out_dtype == torch.float32)
+        return ref.mxfp4_matmul(x, w, out_dtype)
+    _need(x.dim() == 2 and x.shape[1] == w.k,
+          'x must be (N,%d), not %s' % (w.k, tuple(x.shape)))
+    _need(x.device == w.codes.device, 'x and w must be on one device')
+    if backend_for(w.codes) == 'hip':
+        return hip_ext(True).mxfp4_matmul(x, torch.empty(0), w.codes, w.scales,
+                                          w.k, out_dtype == torch.float32)
+    return ref.mxfp4_matmul(x, w, out_dtype)
 
 
 def grad_weight_gemm(ctx, d_z):

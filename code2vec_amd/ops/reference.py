@@ -11,7 +11,7 @@ the identical mask from (seed, element-index).
 """
 
 import math
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -92,6 +92,127 @@ def transform_tanh_bwd(ctx: torch.Tensor, w: torch.Tensor, y: torch.Tensor,
     d_ctx = d_z @ w.to(d_z.dtype).t()
     d_w = (ctx.t().float() @ d_z.float())
     return d_ctx, d_w
+
+
+# ---------------------------------------------------------------------------
+# gated transform: y = act(ctx Wg) * (ctx Wu)
+# ---------------------------------------------------------------------------
+
+GATE_ACTIVATIONS = ('silu', 'gelu', 'sigmoid', 'tanh', 'relu')
+
+
+def gate_activation(name: str, g: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(act(g), act'(g)). gelu is the exact one (with erf); relu'(0) = 0."""
+    if name == 'silu':
+        s = torch.sigmoid(g)
+        return g * s, s * (1.0 + g * (1.0 - s))
+    if name == 'gelu':
+        cdf = 0.5 * (1.0 + torch.erf(g * math.sqrt(0.5)))
+        return g * cdf, cdf + g * torch.exp(-0.5 * g * g) / math.sqrt(2.0 * math.pi)
+    if name == 'sigmoid':
+        s = torch.sigmoid(g)
+        return s, s * (1.0 - s)
+    if name == 'tanh':
+        t = torch.tanh(g)
+        return t, 1.0 - t * t
+    if name == 'relu':
+        return torch.relu(g), (g > 0).to(g.dtype)
+    raise ValueError('unknown activation %r' % (name,))
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def transform_gated_fwd(ctx: torch.Tensor, w_oi: torch.Tensor, activation: str,
+                        save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """ctx (N,K), w_oi (2,H,K): y (N,H), and (N,2,Hp) g and u in ctx's type
+    (rows padded to a multiple of eight, as the kernels keep them) if they
+    are to be kept for the backward."""
+    x, w = _wide(ctx), _wide(w_oi)
+    g, u = x @ w[0].t(), x @ w[1].t()
+    y = (gate_activation(activation, g)[0] * u).to(ctx.dtype)
+    if not save:
+        return y, None
+    gu = torch.nn.functional.pad(torch.stack((g, u), 1), (0, -w.shape[1] % 8))
+    return y, gu.to(ctx.dtype)
+
+
+def transform_gated_bwd(ctx: torch.Tensor, w_io: torch.Tensor, gu: torch.Tensor,
+                        d_y: torch.Tensor, activation: str
+                        ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """w_io (K,2H), gu from the forward: d_ctx (N,K) and d_w (2,K,H), in
+    ctx's type. dg = dy u act'(g); du = dy act(g); d_ctx = [dg|du] w_io^T;
+    d_w = ctx^T [dg|du]."""
+    H = d_y.shape[1]
+    g, u, dy = _wide(gu[:, 0, :H]), _wide(gu[:, 1, :H]), _wide(d_y)
+    a, da = gate_activation(activation, g)
+    dgu = torch.cat((dy * u * da, dy * a), 1)                  # (N, 2H)
+    d_ctx = dgu @ _wide(w_io).t()
+    d_w = _wide(ctx).t() @ dgu                                 # (K, 2H)
+    d_w = d_w.reshape(ctx.shape[1], 2, H).permute(1, 0, 2).contiguous()
+    return d_ctx.to(ctx.dtype), d_w.to(ctx.dtype)
+
+
+# ---------------------------------------------------------------------------
+# MXFP4: blocks of 32 4-bit codes under one power of two
+# ---------------------------------------------------------------------------
+
+MXFP4_BLOCK = 32
+MXFP4_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+class Mxfp4(NamedTuple):
+    """Rows of `k` values in MXFP4. codes (rows, 16*blocks) uint8: two codes a
+    byte, the even value in the low half (bit 3 of a code is its sign, bits
+    0-2 index MXFP4_VALUES). scales (rows, blocks) uint8: 2^(byte-127), 255
+    for a block that held a NaN or an infinity. blocks = ceil(k/32); what
+    fills up the last one is zero."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    k: int
+
+
+def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
+    """Scale of a block: the power of two of its largest magnitude, less two,
+    so that this value lands in 4..8 and is held to 6 at most. Values go to
+    the nearest code, from a middle to the even one."""
+    k = x.shape[1]
+    v = torch.nn.functional.pad(x.float(), (0, -k % MXFP4_BLOCK))
+    v = v.reshape(x.shape[0], -1, MXFP4_BLOCK)
+    bits = v.contiguous().view(torch.int32).bitwise_and(0x7FFFFFFF)
+    field = (bits.amax(-1) if v.numel() else bits.new_zeros(v.shape[:2])) >> 23
+    byte = torch.where(field == 255, field, (field - 2).clamp_min(0))
+    # 2^(127 - byte) in 64 bits: it has no 32-bit normal form at both ends
+    size = (v.double() * torch.exp2(127.0 - byte.double()).unsqueeze(-1)).abs()
+    code = torch.zeros_like(bits)
+    for lo, hi, tie_up in ((0.0, 0.5, False), (0.5, 1.0, True), (1.0, 1.5, False),
+                           (1.5, 2.0, True), (2.0, 3.0, False), (3.0, 4.0, True),
+                           (4.0, 6.0, False)):
+        mid = (lo + hi) / 2
+        code += (size >= mid) if tie_up else (size > mid)
+    code += torch.signbit(v).int() * 8
+    code = torch.where((byte == 255).unsqueeze(-1), torch.zeros_like(code), code)
+    code = code.to(torch.uint8)
+    codes = (code[..., 0::2] | (code[..., 1::2] << 4)).reshape(x.shape[0], -1)
+    return Mxfp4(codes, byte.to(torch.uint8), k)
+
+
+def mxfp4_dequantize(q: Mxfp4, dtype=torch.float32) -> torch.Tensor:
+    rows, blocks = q.scales.shape
+    code = torch.stack((q.codes & 15, q.codes >> 4), -1).long()
+    table = torch.tensor(MXFP4_VALUES + tuple(-v for v in MXFP4_VALUES),
+                         dtype=torch.float64, device=q.codes.device)
+    scale = torch.exp2(q.scales.double() - 127.0)
+    scale = torch.where(q.scales == 255, torch.full_like(scale, math.nan), scale)
+    v = table[code].reshape(rows, blocks, MXFP4_BLOCK) * scale.unsqueeze(-1)
+    return v.reshape(rows, -1)[:, :q.k].to(dtype)
+
+
+def mxfp4_matmul(x, w: Mxfp4, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """x (N,K), a tensor or Mxfp4, times the transpose of w (M,K)."""
+    xf = mxfp4_dequantize(x) if isinstance(x, Mxfp4) else _wide(x)
+    return (xf @ mxfp4_dequantize(w, xf.dtype).t()).to(out_dtype)
 
 
 # ---------------------------------------------------------------------------
