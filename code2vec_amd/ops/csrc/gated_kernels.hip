@@ -20,31 +20,38 @@ namespace {
 
 enum Activation : int { SILU = 0, GELU = 1, SIGMOID = 2, TANH = 3, RELU = 4 };
 
-template <int ACT>
-DEVI float act_fwd(float g) {
-  if constexpr (ACT == SILU) return g / (1.f + __expf(-g));
-  if constexpr (ACT == GELU) return 0.5f * g * (1.f + erff(g * 0.70710678f));
-  if constexpr (ACT == SIGMOID) return 1.f / (1.f + __expf(-g));
-  if constexpr (ACT == TANH) return tanhf(g);
-  return g > 0.f ? g : (g != g ? g : 0.f);
+// The reciprocal and the exponential of the hardware are off by about one
+// step of fp32; their limits are right: 1 / (1 + exp(200)) is zero.
+DEVI float sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.f + __expf(-g));
 }
 
-// act(g) and act'(g)
+// 1 - 2 / (exp(2g) + 1) loses what is small next to one, so that near zero
+// the series takes over: its next term is below 2e-9 of the result
+DEVI float tanh_of(float g) {
+  const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * g));
+  const float s = g * g;
+  const float near = g + g * s * (-0.33333333f + s * (0.13333333f - s * 0.05396825f));
+  return fabsf(g) < 0.125f ? near : far;
+}
+
+// act(g) and act'(g); the derivative costs nothing where it is not used
 template <int ACT>
 DEVI void act_both(float g, float& a, float& da) {
   if constexpr (ACT == SILU) {
-    const float s = 1.f / (1.f + __expf(-g));
+    const float s = sigmoid(g);
     a = g * s;
     da = s * (1.f + g * (1.f - s));
   } else if constexpr (ACT == GELU) {
-    const float cdf = 0.5f * (1.f + erff(g * 0.70710678f));
+    // erfc and not 1 + erf: far left the sum would leave no digits
+    const float cdf = 0.5f * erfcf(g * -0.70710678f);
     a = g * cdf;
     da = cdf + g * __expf(-0.5f * g * g) * 0.39894228f;
   } else if constexpr (ACT == SIGMOID) {
-    a = 1.f / (1.f + __expf(-g));
+    a = sigmoid(g);
     da = a * (1.f - a);
   } else if constexpr (ACT == TANH) {
-    a = tanhf(g);
+    a = tanh_of(g);
     da = 1.f - a * a;
   } else {
     a = g > 0.f ? g : (g != g ? g : 0.f);
@@ -52,7 +59,14 @@ DEVI void act_both(float g, float& a, float& da) {
   }
 }
 
-DEVI void to_lds16(const ushort* src, ushort* dst) {
+// keeps a base in scalar registers, so that a load adds its 32-bit offset
+// by itself and the vector units are left to the epilogue
+DEVI const char* in_scalar(const char* p) {
+  asm("" : "+s"(p));
+  return p;
+}
+
+DEVI void to_lds16(const void* src, ushort* dst) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) u32*)src,
       (__attribute__((address_space(3))) u32*)dst, 16, 0, 0);
@@ -80,7 +94,21 @@ DEVI u16x8 pack8(const float* v) {
 // product.
 // ---------------------------------------------------------------------------
 
-constexpr int BK = 64;   // reduction values a step: rows of 128 bytes in LDS
+// Tiles go from memory into a ring of LDS buffers, STAGES - 1 steps ahead of
+// the matrix instructions. A step begins when its own tile has arrived, which
+// is when no more than the `younger` loads issued after it are outstanding,
+// and when every wave has read the tile that the step's new loads overwrite.
+template <int PER_TILE, int STAGES>
+DEVI void wait_tile(int left) {   // left: steps after this one
+  static_assert(PER_TILE < 64 && (STAGES == 2 || STAGES == 3), "vmcnt has 6 bits");
+  // vmcnt in bits 3:0 and 15:14, expcnt 6:4 (no wait), lgkmcnt 11:8 (zero)
+  constexpr int none = 0x70, one = 0x70 | (PER_TILE & 15) | (PER_TILE >> 4 << 14);
+  asm volatile("" ::: "memory");
+  if (STAGES == 3 && left > 0) __builtin_amdgcn_s_waitcnt(one);
+  else __builtin_amdgcn_s_waitcnt(none);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 enum Epilogue : int { GATED = 0, PLAIN = 1 };
 
@@ -96,8 +124,9 @@ struct BtArgs {
   const long* seed_ptr;
 };
 
-template <int EPI, int ACT, int WR, int WC, int XT, int GT>
-__launch_bounds__(WR * WC * 64)
+template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK,
+          int STAGES>
+__launch_bounds__(WR * WC * 64, 2)
 __global__ void k_rows_gemm(BtArgs p) {
   constexpr int T = WR * WC * 64;
   constexpr int BM = WR * XT * 16;         // rows of x a block
@@ -106,8 +135,11 @@ __global__ void k_rows_gemm(BtArgs p) {
   constexpr int HT = EPI == GATED ? BG : BN;   // output columns a block
   constexpr int CH = BK / 8;               // 16-byte chunks a row
   constexpr int IT = (BM + BN) * CH / T;
-  static_assert((BM + BN) * CH % T == 0 && BM * CH % 64 == 0, "staging");
-  extern __shared__ ushort lds[];          // 2 x (BM + BN) x BK
+  // where a row's 16-byte chunks lie: 8 rows read at once cover all banks
+  auto place = [](int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; };
+  constexpr int ITX = BM * CH / T;         // of them from x
+  static_assert(BM * CH % T == 0 && BN * CH % T == 0, "staging");
+  extern __shared__ ushort lds[];          // STAGES x (BM + BN) x BK
 
   const int nC = (p.H + HT - 1) / HT;
   const int wg = xcd_chunked(blockIdx.x, gridDim.x);
@@ -119,17 +151,17 @@ __global__ void k_rows_gemm(BtArgs p) {
   const int wr = wid / WC, wc = wid % WC;
   const int l16 = lane & 15, q = lane >> 4;
 
-  // this thread's source rows, one for each chunk that it stages
-  const ushort* src[IT];
-  int col[IT];
+  // Where each of this thread's chunks comes from: bytes behind the tile's
+  // first row of x, or behind w. A step adds to the bases alone.
+  u32 off[IT];
 #pragma unroll
   for (int it = 0; it < IT; ++it) {
     const int c = it * T + tid;
     const int r = c / CH, pos = c % CH;
-    col[it] = (pos ^ (r & 7)) * 8;
-    if (r < BM) {
-      const long n = min(row0 + r, (long)p.N - 1);
-      src[it] = p.x + n * p.ldx;
+    const u32 col = (pos ^ place(r)) * 16;
+    if (it < ITX) {
+      const long n = min((long)r, (long)p.N - 1 - row0);
+      off[it] = (u32)(n * p.ldx * 2) + col;
     } else {
       const int j = r - BM;                       // row of w in LDS
       const int i = j & 15, mi = (j >> 4) % GT;
@@ -140,15 +172,27 @@ __global__ void k_rows_gemm(BtArgs p) {
         wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
       else
         wrow = min(h0 + (cw * 2 + grp) * GT * 16 + in_group, p.H - 1);
-      src[it] = p.w + wrow * p.K;
+      off[it] = (u32)(wrow * p.K * 2) + col;
     }
   }
+  const char* xb = reinterpret_cast<const char*>(p.x + row0 * p.ldx);
+  const char* wb = reinterpret_cast<const char*>(p.w);
   auto stage = [&](int k0, int buf) {
+    ushort* dst = lds + buf * (BM + BN) * BK + wid * 512;
+    if (k0 + BK <= p.K) {
+      const char* xk = in_scalar(xb + k0 * 2l);
+      const char* wk = in_scalar(wb + k0 * 2l);
 #pragma unroll
-    for (int it = 0; it < IT; ++it) {
-      const int k = k0 + col[it];
-      const ushort* s = k < p.K ? src[it] + k : k_zero_chunk;
-      to_lds16(s, lds + (long)buf * (BM + BN) * BK + (it * T + wid * 64) * 8);
+      for (int it = 0; it < IT; ++it)
+        to_lds16((it < ITX ? xk : wk) + off[it], dst + it * T * 8);
+    } else {
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        const int r = (it * T + tid) / CH, pos = (it * T + tid) % CH;
+        const char* s = (it < ITX ? xb : wb) + k0 * 2l + off[it];
+        to_lds16(k0 + (pos ^ place(r)) * 8 < p.K ? (const void*)s : k_zero_chunk,
+                 dst + it * T * 8);
+      }
     }
   };
 
@@ -160,15 +204,19 @@ __global__ void k_rows_gemm(BtArgs p) {
 
   const int steps = (p.K + BK - 1) / BK;
   stage(0, 0);
-  __syncthreads();
+  if (STAGES == 3 && steps > 1) stage(BK, 1);
+  int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) stage((s + 1) * BK, (s + 1) & 1);
-    const ushort* xs = lds + (s & 1) * (BM + BN) * BK + wr * XT * 16 * BK;
-    const ushort* ws = lds + (s & 1) * (BM + BN) * BK +
+    wait_tile<IT, STAGES>(steps - 1 - s);
+    if (s + STAGES - 1 < steps)
+      stage((s + STAGES - 1) * BK, buf == 0 ? STAGES - 1 : buf - 1);
+    const ushort* xs = lds + buf * (BM + BN) * BK + wr * XT * 16 * BK;
+    const ushort* ws = lds + buf * (BM + BN) * BK +
                        (BM + wc * 2 * GT * 16) * BK;
+    buf = buf == STAGES - 1 ? 0 : buf + 1;
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
-      const int off = l16 * BK + (((kk * 4 + q) ^ (l16 & 7)) * 8);
+      const int off = l16 * BK + (((kk * 4 + q) ^ place(l16)) * 8);
       bf16x8 xf[XT], wf[2 * GT];
 #pragma unroll
       for (int i = 0; i < XT; ++i)
@@ -183,7 +231,6 @@ __global__ void k_rows_gemm(BtArgs p) {
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               wf[j], xf[i], acc[i][j], 0, 0, 0);
     }
-    __syncthreads();
   }
 
   const bool vec = (p.H & 7) == 0;
@@ -217,7 +264,9 @@ __global__ void k_rows_gemm(BtArgs p) {
         for (int r = 0; r < 4; ++r) {
           gv[j * 4 + r] = acc[i][j][r];
           uv[j * 4 + r] = acc[i][GT + j][r];
-          yv[j * 4 + r] = act_fwd<ACT>(acc[i][j][r]) * acc[i][GT + j][r];
+          float a, da;
+          act_both<ACT>(gv[j * 4 + r], a, da);
+          yv[j * 4 + r] = a * uv[j * 4 + r];
         }
       put(p.y + n * p.H + h, yv, h);
       if (p.gu) {
@@ -298,7 +347,7 @@ __global__ void k_gated_dgu(const ushort* __restrict__ gu,
 // 32 is the same for both operands and does not matter to the sum: lane
 // group q takes rows 4q..4q+3 and 16+4q..16+4q+3, so that one read covers 16
 // neighbouring rows, whose 32-byte units the exclusive-or below spreads over
-// all banks. N is split over gridDim.y; the parts are added in order by
+// all banks. N is split over blocks; the parts are added in order by
 // k_dw_reduce, so that a result never depends on timing.
 // ---------------------------------------------------------------------------
 
@@ -320,11 +369,11 @@ DEVI bf16x8 tr_read(const ushort* tile, int stride, int c0, int l16, int q) {
 }
 
 template <int WA, int WB, int AT, int BT>
-__launch_bounds__(WA * WB * 64)
+__launch_bounds__(WA * WB * 64, 2)
 __global__ void k_dw_part(const ushort* __restrict__ dgu,
                           const ushort* __restrict__ x, long ldx,
                           float* __restrict__ part, int N, int C2, int K,
-                          int K8, int rows_each) {
+                          int K8, int rows_each, int tiles) {
   constexpr int T = WA * WB * 64;
   constexpr int CA = WA * AT * 16;     // columns of dgu a block
   constexpr int CB = WB * BT * 16;     // columns of x a block
@@ -334,8 +383,11 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
   constexpr int BUF = TN_ROWS * (CA + CB);
 
   const int nB = (K + CB - 1) / CB;
-  const int a0 = blockIdx.x / nB * CA, b0 = blockIdx.x % nB * CB;
-  const long n0 = (long)blockIdx.y * rows_each;
+  // the tiles of one part of the rows share an L2
+  const int wg = xcd_chunked(blockIdx.x, gridDim.x);
+  const int tile = wg % tiles, slice = wg / tiles;
+  const int a0 = tile / nB * CA, b0 = tile % nB * CB;
+  const long n0 = (long)slice * rows_each;
   const long n1 = min(n0 + rows_each, (long)N);
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -343,26 +395,39 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
   const int wa = wid / WB, wb = wid % WB;
   const int l16 = lane & 15, q = lane >> 4;
 
+  // bytes behind the step's first row of dgu or of x; columns that are not
+  // there read others, and what becomes of them is not stored
+  u32 off[ITA + ITB];
+#pragma unroll
+  for (int it = 0; it < ITA + ITB; ++it) {
+    const bool ina = it < ITA;
+    const int c = (ina ? it : it - ITA) * T + tid;
+    const int per = (ina ? CA : CB) / 8;
+    const int r = c / per, pos = c % per;
+    const int cc = (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
+    off[it] = ina ? (u32)((long)r * C2 + (a0 + cc < C2 ? a0 + cc : 0)) * 2
+                  : (u32)((long)r * ldx + (b0 + cc < K8 ? b0 + cc : 0)) * 2;
+  }
   auto stage = [&](long n, int buf) {
-    ushort* la = lds + buf * BUF;
-    ushort* lb = la + TN_ROWS * CA;
+    ushort* dst = lds + buf * BUF + wid * 512;
+    const char* ap = reinterpret_cast<const char*>(dgu + n * C2);
+    const char* bp = reinterpret_cast<const char*>(x + n * ldx);
+    if (n + TN_ROWS <= n1) {
+      ap = in_scalar(ap);
+      bp = in_scalar(bp);
 #pragma unroll
-    for (int it = 0; it < ITA; ++it) {
-      const int c = it * T + tid;
-      const int r = c / (CA / 8), pos = c % (CA / 8);
-      const int cc = a0 + (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
-      const ushort* s = (n + r < n1 && cc < C2) ? dgu + (n + r) * C2 + cc
-                                                : k_zero_chunk;
-      to_lds16(s, la + (it * T + wid * 64) * 8);
-    }
+      for (int it = 0; it < ITA + ITB; ++it)
+        to_lds16((it < ITA ? ap : bp) + off[it],
+                 dst + (it < ITA ? it * T * 8 : TN_ROWS * CA + (it - ITA) * T * 8));
+    } else {
 #pragma unroll
-    for (int it = 0; it < ITB; ++it) {
-      const int c = it * T + tid;
-      const int r = c / (CB / 8), pos = c % (CB / 8);
-      const int cc = b0 + (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
-      const ushort* s = (n + r < n1 && cc < K8) ? x + (n + r) * ldx + cc
-                                                : k_zero_chunk;
-      to_lds16(s, lb + (it * T + wid * 64) * 8);
+      for (int it = 0; it < ITA + ITB; ++it) {
+        const bool ina = it < ITA;
+        const int r = ((ina ? it : it - ITA) * T + tid) / ((ina ? CA : CB) / 8);
+        const char* s = (ina ? ap : bp) + off[it];
+        to_lds16(n + r < n1 ? (const void*)s : k_zero_chunk,
+                 dst + (ina ? it * T * 8 : TN_ROWS * CA + (it - ITA) * T * 8));
+      }
     }
   };
 
@@ -374,11 +439,15 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
 
   const int steps = (int)((n1 - n0 + TN_ROWS - 1) / TN_ROWS);
   if (steps > 0) stage(n0, 0);
-  __syncthreads();
+  if (steps > 1) stage(n0 + TN_ROWS, 1);
+  int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps) stage(n0 + (long)(s + 1) * TN_ROWS, (s + 1) & 1);
-    const ushort* la = lds + (s & 1) * BUF;
+    wait_tile<ITA + ITB, 3>(steps - 1 - s);
+    if (s + 2 < steps)
+      stage(n0 + (long)(s + 2) * TN_ROWS, buf == 0 ? 2 : buf - 1);
+    const ushort* la = lds + buf * BUF;
     const ushort* lb = la + TN_ROWS * CA;
+    buf = buf == 2 ? 0 : buf + 1;
     bf16x8 af[AT], bf[BT];
 #pragma unroll
     for (int i = 0; i < AT; ++i)
@@ -392,7 +461,6 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
       for (int j = 0; j < BT; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[i], bf[j],
                                                             acc[i][j], 0, 0, 0);
-    __syncthreads();
   }
   // part (S, K, C2): a lane holds four consecutive columns of C2
 #pragma unroll
@@ -403,7 +471,7 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
     for (int i = 0; i < AT; ++i) {
       const int c = a0 + (wa * AT + i) * 16 + q * 4;
       if (c < C2)
-        *reinterpret_cast<f32x4*>(part + ((long)blockIdx.y * K + k) * C2 + c) =
+        *reinterpret_cast<f32x4*>(part + ((long)slice * K + k) * C2 + c) =
             acc[i][j];
     }
   }
@@ -476,6 +544,12 @@ void check_bf16(const torch::Tensor& t, const char* name, int dims,
   TORCH_CHECK(t.dim() == dims, name, " must have ", dims, " dimensions");
 }
 
+void check_size(long N, long K, long H) {
+  TORCH_CHECK(N < (1L << 31) && K < (1L << 22) && H < (1L << 21) &&
+              (K + 8) * (H + 8) < (1L << 30),
+              "ctx (", N, ", ", K, ") or the weights to ", H, " are too large");
+}
+
 // Rows whose values follow each other, start on 16 bytes and are a multiple
 // of eight long: `t` itself, or a padded copy of it.
 struct Rows {
@@ -487,7 +561,8 @@ struct Rows {
 Rows chunked_rows(const torch::Tensor& t, int cols) {
   const bool dense = t.size(1) <= 1 || t.stride(1) == 1;
   const long ld = t.size(0) <= 1 ? pad8(cols) : t.stride(0);
-  if (dense && cols % 8 == 0 && ld % 8 == 0 && ld >= 0 &&
+  // (offsets within a tile have 32 bits)
+  if (dense && cols % 8 == 0 && ld % 8 == 0 && ld >= 0 && ld < (1l << 23) &&
       (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0)
     return {t, bf_ptr(t), ld};
   auto src = dense ? t : t.contiguous();
@@ -499,12 +574,12 @@ Rows chunked_rows(const torch::Tensor& t, int cols) {
   return {out, bf_ptr(out), (long)pad8(cols)};
 }
 
-template <int EPI, int ACT, int WR, int WC, int XT, int GT>
+template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK, int STAGES>
 void launch_rows(const BtArgs& a) {
   constexpr int BM = WR * XT * 16, BG = WC * GT * 16;
   constexpr int HT = EPI == GATED ? BG : 2 * BG;
-  constexpr size_t bytes = 2ul * (BM + 2 * BG) * BK * sizeof(ushort);
-  auto* fn = &k_rows_gemm<EPI, ACT, WR, WC, XT, GT>;
+  constexpr size_t bytes = (size_t)STAGES * (BM + 2 * BG) * BK * sizeof(ushort);
+  auto* fn = &k_rows_gemm<EPI, ACT, WR, WC, XT, GT, BK, STAGES>;
   if (bytes > 64 * 1024)
     C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
                                        hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -517,7 +592,22 @@ void launch_rows(const BtArgs& a) {
 
 template <int EPI, int ACT>
 void rows_gemm(const BtArgs& a) {
-  launch_rows<EPI, ACT, 4, 2, 4, 4>(a);
+  launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a);
+}
+
+// How many parts the rows are cut into for dW. 512 blocks run at a time: a
+// part more than fills them costs a whole round, and every part costs the
+// writing and reading of its sums.
+int dw_parts(long tiles, long N, long outputs) {
+  int best = 1;
+  double least = 1e30;
+  for (long S = 1; S <= 64 && (S == 1 || N / S >= 256); ++S) {
+    const long rounds = (tiles * S + 511) / 512;
+    const double rows = (double)rounds * (N / S + 96);     // one block's, and its start
+    const double us = rows * 0.030 + (double)S * outputs * 8 / 5e6;
+    if (us < least) { least = us; best = (int)S; }
+  }
+  return best;
 }
 
 template <int ACT>
@@ -547,8 +637,7 @@ std::vector<torch::Tensor> transform_gated_fwd(torch::Tensor ctx,
   check_bf16(w_oi, "w_oi", 3, ctx);
   TORCH_CHECK(w_oi.size(0) == 2 && w_oi.size(2) == ctx.size(1) &&
               w_oi.is_contiguous(), "w_oi must be a contiguous (2, H, K)");
-  TORCH_CHECK(ctx.size(0) < (1L << 31) && ctx.size(1) < (1L << 24) &&
-              w_oi.size(1) < (1L << 24), "ctx or w_oi is too large");
+  check_size(ctx.size(0), ctx.size(1), w_oi.size(1));
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
   const int N = ctx.size(0), K = ctx.size(1), H = w_oi.size(1), Hp = pad8(H);
   auto y = torch::empty({N, H}, ctx.options());
@@ -573,6 +662,7 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   check_bf16(gu, "gu", 3, ctx);
   check_bf16(d_y, "d_y", 2, ctx);
   const int N = ctx.size(0), K = ctx.size(1), H = d_y.size(1), Hp = pad8(H);
+  check_size(ctx.size(0), ctx.size(1), d_y.size(1));
   TORCH_CHECK(d_y.size(0) == N, "d_y must have as many rows as ctx");
   TORCH_CHECK(w_io.size(0) == K && w_io.size(1) == 2L * H && w_io.is_contiguous(),
               "w_io must be a contiguous (K, 2H)");
@@ -616,15 +706,16 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   constexpr int WA = 2, WB = 2, AT = 8, BT = 4;
   const int tiles = (2 * Hp + WA * AT * 16 - 1) / (WA * AT * 16) *
                     ((K + WB * BT * 16 - 1) / (WB * BT * 16));
-  const long most = ((long)N + 255) / 256;   // at least 256 rows a part
-  const int S = (int)std::max(1L, std::min(most, (long)(512 + tiles - 1) / tiles));
+  const int S = dw_parts(tiles, N, (long)K * 2 * Hp);
   const int rows_each = (int)((((long)N + S - 1) / S + TN_ROWS - 1) / TN_ROWS * TN_ROWS);
   auto part = torch::empty({S, K, 2L * Hp}, ctx.options().dtype(torch::kFloat32));
-  constexpr size_t bytes = 2ul * TN_ROWS * (WA * AT + WB * BT) * 16 * sizeof(ushort);
+  constexpr size_t bytes = 3ul * TN_ROWS * (WA * AT + WB * BT) * 16 * sizeof(ushort);
   auto* dw = &k_dw_part<WA, WB, AT, BT>;
-  dw<<<dim3(tiles, S), WA * WB * 64, bytes, cur_stream()>>>(
+  C10_HIP_CHECK(hipFuncSetAttribute(
+      (const void*)dw, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  dw<<<tiles * S, WA * WB * 64, bytes, cur_stream()>>>(
       bf_ptr(dgu), x.p, x.ld, part.data_ptr<float>(), N, 2 * Hp, K, pad8(K),
-      rows_each);
+      rows_each, tiles);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   auto d_w = torch::empty({2, K, H}, ctx.options());
   const long quads = (long)K * 2 * Hp / 4;

@@ -156,6 +156,12 @@ __global__ void k_mxfp4_dequantize(const u32* __restrict__ codes,
 //
 // Lane (i, q) holds block 4s + q of its row in step s of 128 values: for x in
 // bf16 sub-step j multiplies values 8j..8j+7 of that block.
+//
+// Large products are bound by writing y, and y's rows need not start on a
+// cache line. Lines that are written in two halves halve the rate, so a tile
+// takes rows that all lie the same way: every `period`-th one. The columns of
+// its passes then begin on lines, `shift` columns before those of row 0 of
+// the table (the first pass has columns below zero, which are not stored).
 // ---------------------------------------------------------------------------
 
 struct MxArgs {
@@ -168,42 +174,49 @@ struct MxArgs {
   void* y;                    // (N, M)
   int N, M, K, nb;
   int kc;                     // values of a row of x in LDS, a multiple of 128
-  int n_tiles, slices;        // blocks: n_tiles x slices
-  int chunks_each;            // chunks of w rows a slice
+  int period, n_tiles;        // tiles of x: n_tiles, a multiple of period
+  int chunks_each;            // passes over rows of w a block
   int vec;                    // x can be read 16 bytes at a time
 };
 
+constexpr int MX_WAVES = 4;
+
 template <bool X4, bool OUT32, int XT, int MT>
-__launch_bounds__(512, 2)
+__launch_bounds__(MX_WAVES * 64, XT == 1 ? 4 : 3)
 __global__ void k_mxfp4_rows(MxArgs p) {
-  constexpr int WAVES = 8, T = WAVES * 64;
-  constexpr int ROWS = XT * 16;             // rows of x a block
-  constexpr int CHUNK = WAVES * MT * 16;    // rows of w a pass
+  constexpr int T = MX_WAVES * 64;
+  constexpr int ROWS = XT * 16;                // rows of x a block
+  constexpr int CHUNK = MX_WAVES * MT * 16;    // rows of w a pass
+  constexpr int ES = OUT32 ? 4 : 2;
   extern __shared__ uint8_t sm[];
   // an odd number of 16-byte units a row, so that 8 rows lie on all banks
   const int stride = (X4 ? p.kc / 2 : p.kc * 2) + 16;
-  uint8_t* sm_scales = sm + ROWS * stride;  // X4: (ROWS, kc / 32)
   const int kb = p.kc / 32;
+  uint8_t* sm_scales = sm + ROWS * stride;     // X4: (ROWS, kb)
 
   const int b = xcd_chunked(blockIdx.x, gridDim.x);
-  const int slice = b / p.n_tiles;
-  const int n0 = (b % p.n_tiles) * ROWS;
+  const int tile = b % p.n_tiles;
+  const int n0 = tile % p.period + tile / p.period * ROWS * p.period;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, q = lane >> 4;
-  const int row_in = (l16 >> 2) * (4 * MT) + (l16 & 3);
 
-  const int k_chunks = (p.nb * 32 + p.kc - 1) / p.kc;
+  const int shift = p.period == 1 ? 0 :
+      (int)(((u64)p.y + (u64)n0 * p.M * ES) & 127) / ES;
+  const int chunks = (p.M + shift + CHUNK - 1) / CHUNK;
+  const int chunk0 = b / p.n_tiles * p.chunks_each;
+  const int chunk1 = min(chunk0 + p.chunks_each, chunks);
+  const int k_chunks = (p.nb + kb - 1) / kb;
 
-  auto stage = [&](int kc0) {   // x[n0.., kc0 .. kc0 + kc) into LDS
+  auto stage = [&](int b0) {    // blocks b0 .. b0 + kb of the rows into LDS
     if constexpr (X4) {
-      const int b0 = kc0 / 32;
       for (int c = tid; c < ROWS * kb; c += T) {
         const int r = c / kb, blk = c % kb;
+        const long n = n0 + (long)r * p.period;
         u32x4 v = {0u, 0u, 0u, 0u};
         uint8_t s = 127;
-        if (n0 + r < p.N && b0 + blk < p.nb) {
-          const long at = (long)(n0 + r) * p.nb + b0 + blk;
+        if (n < p.N && b0 + blk < p.nb) {
+          const long at = n * p.nb + b0 + blk;
           v = *reinterpret_cast<const u32x4*>(p.xc + at * 16);
           s = p.xs[at];
         }
@@ -213,129 +226,107 @@ __global__ void k_mxfp4_rows(MxArgs p) {
     } else {
       const int c8 = p.kc / 8;
       for (int c = tid; c < ROWS * c8; c += T) {
-        const int r = c / c8, k = c % c8 * 8;
+        const int r = c / c8, k = b0 * 32 + c % c8 * 8;
+        const long n = n0 + (long)r * p.period;
         u16x8 v = {};
-        if (n0 + r < p.N) {
-          const ushort* s = p.x + (long)(n0 + r) * p.ldx + kc0 + k;
-          if (p.vec && kc0 + k + 8 <= p.K) {
+        if (n < p.N) {
+          const ushort* s = p.x + n * p.ldx + k;
+          if (p.vec && k + 8 <= p.K) {
             v = *reinterpret_cast<const u16x8*>(s);
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (kc0 + k + j < p.K) v[j] = s[j];
+            for (int j = 0; j < 8; ++j) if (k + j < p.K) v[j] = s[j];
           }
         }
-        *reinterpret_cast<u16x8*>(sm + r * stride + k * 2) = v;
-      }
-    }
-  };
-  auto load_w = [&](int m0, int blk, u32x4* c, u32* s) {
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const long m = min(m0 + row_in + t * 4, p.M - 1);
-      if (blk < p.nb) {
-        c[t] = *reinterpret_cast<const u32x4*>(p.wc + (m * p.nb + blk) * 16);
-        s[t] = p.ws[m * p.nb + blk];
-      } else {
-        c[t] = u32x4{0u, 0u, 0u, 0u};
-        s[t] = 127;
+        *reinterpret_cast<u16x8*>(sm + r * stride + c % c8 * 16) = v;
       }
     }
   };
 
-  const int chunk0 = slice * p.chunks_each;
-  const int chunks = (p.M + CHUNK - 1) / CHUNK;
-  const int chunk1 = min(chunk0 + p.chunks_each, chunks);
-  for (int ch = chunk0; ch < chunk1; ++ch) {
-    const int m0 = ch * CHUNK + wid * MT * 16;
-    f32x4 acc[XT][MT];
+  // Rows of w of this lane in a pass, and what it holds of them in a step.
+  // A step behind a row's last block repeats that block's codes: x has zeros
+  // there, and the scale is made harmless.
+  const int row_in = wid * MT * 16 + (l16 >> 2) * (4 * MT) + (l16 & 3);
+  struct Held { u32x4 c[MT]; u32 s[MT]; };
+  auto load = [&](int ch, int blk, Held& h) {
+    const int m0 = ch * CHUNK - shift + row_in;
+    const int at = min(blk, p.nb - 1);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const u64 i = (u64)max(0, min(m0 + t * 4, p.M - 1)) * p.nb + at;
+      h.c[t] = *reinterpret_cast<const u32x4*>(p.wc + i * 16);
+      const u32 s = p.ws[i];
+      h.s[t] = blk < p.nb ? s : 127;
+    }
+  };
+
+  f32x4 acc[XT][MT];
+  auto clear = [&] {
 #pragma unroll
     for (int i = 0; i < XT; ++i)
 #pragma unroll
       for (int t = 0; t < MT; ++t) acc[i][t] = {0.f, 0.f, 0.f, 0.f};
-
-    for (int kc = 0; kc < k_chunks; ++kc) {
-      u32x4 wq[2][MT];
-      u32 sq[2][MT];
-      const int b0 = kc * kb;
-      const int steps = (min(kb, p.nb - b0) + 3) / 4;
-      load_w(m0, b0 + q, wq[0], sq[0]);
-      if (ch == chunk0 || k_chunks > 1) {
-        if (ch != chunk0 || kc) __syncthreads();
-        stage(kc * p.kc);
-        __syncthreads();
+  };
+  auto step = [&](int s, const Held& h) {
+    if constexpr (X4) {
+      i32x8 xf[XT];
+      int xsc[XT];
+#pragma unroll
+      for (int i = 0; i < XT; ++i) {
+        const int r = i * 16 + l16;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(
+            sm + r * stride + (s * 4 + q) * 16);
+        xf[i] = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+        xsc[i] = sm_scales[r * kb + s * 4 + q];
       }
-      auto step = [&](int s, const u32x4* wv, const u32* sv) {
-        if constexpr (X4) {
-          i32x8 xf[XT];
-          int xsc[XT];
 #pragma unroll
-          for (int i = 0; i < XT; ++i) {
-            const int r = i * 16 + l16;
-            const u32x4 v = *reinterpret_cast<const u32x4*>(
-                sm + r * stride + (s * 4 + q) * 16);
-            xf[i] = i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
-            xsc[i] = sm_scales[r * kb + s * 4 + q];
-          }
+      for (int t = 0; t < MT; ++t) {
+        const i32x8 wf = {(int)h.c[t][0], (int)h.c[t][1], (int)h.c[t][2],
+                          (int)h.c[t][3], 0, 0, 0, 0};
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const i32x8 wf = {(int)wv[t][0], (int)wv[t][1], (int)wv[t][2],
-                              (int)wv[t][3], 0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < XT; ++i)
-              acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                  wf, xf[i], acc[i][t], 4, 4, 0, (int)sv[t], 0, xsc[i]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // one sub-step's operands at a time: hoisted together they spill
-            __builtin_amdgcn_sched_barrier(0);
-            bf16x8 xf[XT];
-#pragma unroll
-            for (int i = 0; i < XT; ++i)
-              xf[i] = *reinterpret_cast<const bf16x8*>(
-                  sm + (i * 16 + l16) * stride + (s * 128 + q * 32 + j * 8) * 2);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              const bf16x8 wf = decode8(wv[t][j], scale_of(sv[t]));
-#pragma unroll
-              for (int i = 0; i < XT; ++i)
-                acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    wf, xf[i], acc[i][t], 0, 0, 0);
-            }
-          }
-        }
-      };
-      int s = 0;
-#pragma unroll 1
-      for (; s + 1 < steps; s += 2) {
-        load_w(m0, b0 + (s + 1) * 4 + q, wq[1], sq[1]);
-        step(s, wq[0], sq[0]);
-        if (s + 2 < steps) load_w(m0, b0 + (s + 2) * 4 + q, wq[0], sq[0]);
-        step(s + 1, wq[1], sq[1]);
+        for (int i = 0; i < XT; ++i)
+          acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              wf, xf[i], acc[i][t], 4, 4, 0, (int)h.s[t], 0, xsc[i]);
       }
-      if (s < steps) step(s, wq[0], sq[0]);
-    }
-
+    } else {
 #pragma unroll
-    for (int i = 0; i < XT; ++i) {
-      const int n = n0 + i * 16 + l16;
-      if (n >= p.N) continue;
-      const int m = m0 + q * 4 * MT;
-      if constexpr (OUT32) {
-        float* o = reinterpret_cast<float*>(p.y) + (long)n * p.M + m;
+      for (int j = 0; j < 4; ++j) {
+        bf16x8 xf[XT];
+#pragma unroll
+        for (int i = 0; i < XT; ++i)
+          xf[i] = *reinterpret_cast<const bf16x8*>(
+              sm + (i * 16 + l16) * stride + (s * 128 + q * 32 + j * 8) * 2);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          if (m + t * 4 + 4 <= p.M) {
+          const bf16x8 wf = decode8(h.c[t][j], scale_of(h.s[t]));
+#pragma unroll
+          for (int i = 0; i < XT; ++i)
+            acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                wf, xf[i], acc[i][t], 0, 0, 0);
+        }
+      }
+    }
+  };
+  auto store = [&](int ch) {
+    const int m = ch * CHUNK - shift + wid * MT * 16 + q * 4 * MT;
+#pragma unroll
+    for (int i = 0; i < XT; ++i) {
+      const long n = n0 + (long)(i * 16 + l16) * p.period;
+      if (n >= p.N) continue;
+      if constexpr (OUT32) {
+        float* o = reinterpret_cast<float*>(p.y) + n * p.M + m;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          if (m + t * 4 >= 0 && m + t * 4 + 4 <= p.M) {
             *reinterpret_cast<f32x4_any*>(o + t * 4) = acc[i][t];
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (m + t * 4 + r < p.M) o[t * 4 + r] = acc[i][t][r];
+              if ((u32)(m + t * 4 + r) < (u32)p.M) o[t * 4 + r] = acc[i][t][r];
           }
         }
       } else {
-        ushort* o = reinterpret_cast<ushort*>(p.y) + (long)n * p.M + m;
+        ushort* o = reinterpret_cast<ushort*>(p.y) + n * p.M + m;
 #pragma unroll
         for (int t = 0; t < MT; t += 2) {
           bf16x8 v8;
@@ -345,15 +336,56 @@ __global__ void k_mxfp4_rows(MxArgs p) {
             v8[4 + r] = (__bf16)acc[i][t + 1][r];
           }
           const u16x8 v = __builtin_bit_cast(u16x8, v8);
-          if (m + t * 4 + 8 <= p.M) {
+          if (m + t * 4 >= 0 && m + t * 4 + 8 <= p.M) {
             *reinterpret_cast<u16x8_any*>(o + t * 4) = v;
           } else {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
-              if (m + t * 4 + r < p.M) o[t * 4 + r] = v[r];
+              if ((u32)(m + t * 4 + r) < (u32)p.M) o[t * 4 + r] = v[r];
           }
         }
       }
+    }
+  };
+
+  if (chunk0 >= chunk1) return;
+  // one step ahead of the matrix instructions, over the ends of passes
+  Held now, next;
+  load(chunk0, q, now);
+  if (k_chunks == 1) {
+    const int steps = (p.nb + 3) / 4;
+    stage(0);
+    __syncthreads();
+    for (int ch = chunk0; ch < chunk1; ++ch) {
+      clear();
+#pragma unroll 1
+      for (int s = 0; s < steps; ++s) {
+        const bool end = s + 1 == steps;
+        // behind the last pass: its rows once more
+        load(end ? min(ch + 1, chunk1 - 1) : ch, (end ? 0 : s + 1) * 4 + q, next);
+        step(s, now);
+        now = next;
+      }
+      store(ch);
+    }
+  } else {
+    for (int ch = chunk0; ch < chunk1; ++ch) {
+      clear();
+      for (int b0 = 0; b0 < p.nb; b0 += kb) {
+        __syncthreads();
+        stage(b0);
+        __syncthreads();
+        const int steps = (min(kb, p.nb - b0) + 3) / 4;
+#pragma unroll 1
+        for (int s = 0; s < steps; ++s) {
+          const int blk = b0 + (s + 1) * 4;
+          const bool end = blk >= p.nb;
+          load(end ? min(ch + 1, chunk1 - 1) : ch, (end ? 0 : blk) + q, next);
+          step(s, now);
+          now = next;
+        }
+      }
+      store(ch);
     }
   }
 }
@@ -411,7 +443,7 @@ void check_mx(const torch::Tensor& codes, const torch::Tensor& scales, long K,
   TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous() &&
               (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0,
               name, " must be contiguous and start on 16 bytes");
-  TORCH_CHECK(codes.size(0) < (1L << 31) && K < (1L << 30), name, " is too large");
+  TORCH_CHECK(codes.size(0) < (1L << 30) && K < (1L << 30), name, " is too large");
 }
 
 torch::Tensor mxfp4_dequantize(torch::Tensor codes, torch::Tensor scales,
@@ -433,31 +465,40 @@ torch::Tensor mxfp4_dequantize(torch::Tensor codes, torch::Tensor scales,
 
 template <bool X4, bool OUT32, int XT, int MT>
 void launch_mx(MxArgs a) {
-  constexpr int ROWS = XT * 16, CHUNK = 8 * MT * 16;
+  constexpr int ROWS = XT * 16, CHUNK = MX_WAVES * MT * 16;
   // what of a row of x fits LDS: all of it, or a part
-  const int most = X4 ? 2048 : 1024;
-  const int k_all = (a.nb * 32 + 127) / 128 * 128;
-  a.kc = std::min(k_all, most);
+  const int most = X4 ? 2048 : (XT == 4 ? 512 : 1024);
+  a.kc = std::min((a.nb * 32 + 127) / 128 * 128, most);
   const size_t bytes = (size_t)ROWS * ((X4 ? a.kc / 2 : a.kc * 2) + 16) +
                        (X4 ? (size_t)ROWS * (a.kc / 32) : 0);
-  a.n_tiles = (a.N + ROWS - 1) / ROWS;
-  const int chunks = (a.M + CHUNK - 1) / CHUNK;
-  const int want = std::max(1, (512 + a.n_tiles - 1) / a.n_tiles);
-  a.chunks_each = std::max(1, (chunks + want - 1) / want);
-  a.slices = (chunks + a.chunks_each - 1) / a.chunks_each;
+  const int per = (a.N + a.period - 1) / a.period;
+  a.n_tiles = a.period * ((per + ROWS - 1) / ROWS);
+  const int chunks = (int)(((long)a.M + (a.period > 1 ? 63 : 0) + CHUNK - 1) / CHUNK);
+  const int want = std::max(1, (768 + a.n_tiles - 1) / a.n_tiles);
+  a.chunks_each = (chunks + want - 1) / want;
+  const long blocks = (long)a.n_tiles * ((chunks + a.chunks_each - 1) / a.chunks_each);
   auto* fn = &k_mxfp4_rows<X4, OUT32, XT, MT>;
   if (bytes > 64 * 1024)
     C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
                                       hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      160 * 1024));
-  TORCH_CHECK((long)a.n_tiles * a.slices < (1L << 31), "too many tiles");
-  fn<<<a.n_tiles * a.slices, 512, bytes, cur_stream()>>>(a);
+                                      (int)bytes));
+  TORCH_CHECK(blocks < (1L << 31), "too many tiles");
+  fn<<<(int)blocks, MX_WAVES * 64, bytes, cur_stream()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
 template <bool X4, bool OUT32>
-void pick_mx(const MxArgs& a) {
-  if (a.N <= 16) launch_mx<X4, OUT32, 1, 4>(a);
+void pick_mx(MxArgs a) {
+  // rows this many apart start on the same place of a 128-byte line
+  const int over = (int)((long)a.M * (OUT32 ? 4 : 2) % 128);
+  a.period = 1;
+  for (int v = 128; over && v > 1 && over % v; v /= 2) a.period *= 2;
+  if (a.N < 16 * a.period) a.period = 1;     // too few of them for a tile
+  // a tile costs its rows, and about as much as 16 for the rows of w
+  const int per = (a.N + a.period - 1) / a.period;
+  auto cost = [&](int xt) { return (per + 16 * xt - 1) / (16 * xt) * (16 * xt + 16); };
+  if (cost(1) <= cost(2) && cost(1) <= cost(4)) launch_mx<X4, OUT32, 1, 4>(a);
+  else if (cost(2) <= cost(4)) launch_mx<X4, OUT32, 2, 4>(a);
   else launch_mx<X4, OUT32, 4, 4>(a);
 }
 
@@ -478,7 +519,7 @@ torch::Tensor mxfp4_matmul(torch::Tensor x, torch::Tensor x_scales,
   } else {
     TORCH_CHECK(x.scalar_type() == torch::kBFloat16 && x.dim() == 2 &&
                 x.size(1) == K, "x must be a bfloat16 (N, K)");
-    TORCH_CHECK(x.size(0) < (1L << 31), "x is too large");
+    TORCH_CHECK(x.size(0) < (1L << 30), "x is too large");
     if (K > 1 && x.stride(1) != 1) src = x.contiguous();
     a.x = reinterpret_cast<const ushort*>(src.data_ptr<at::BFloat16>());
     a.ldx = x.size(0) == 1 ? K : src.stride(0);
