@@ -216,7 +216,8 @@ struct MxArgs {
   int N, M, K, nb;
   int kc;                     // values of a row of x in LDS, a multiple of 128
   int n_tiles;                // tiles of rows of x
-  int passes_each;            // passes over rows of w a block
+  int passes, passes_each;    // passes over rows of w, in all and a block
+  int period;                 // rows of y this many apart lie alike on lines
   int vec;                    // x can be read 16 bytes at a time
 };
 
@@ -416,137 +417,145 @@ __global__ void k_mxfp4_rows(MxArgs p) {
 // the writes. So:
 //
 // A wave holds its 16*XT rows of x in registers for good, and rows of w are
-// what moves: 64 at a time, through a ring of LDS buffers that the block's
-// eight waves share, so that w is read once for 128*XT rows of x.
+// what moves: 64 at a time, through a ring of four LDS buffers that the
+// block's eight waves share, so that w is read once for 128*XT rows of x.
 //
-// Lines of y that are written in two halves cost twice (measured on 2.1 GB:
-// 950 us as the lanes hold them, 500 us as whole rows of 512, 405 us as whole
-// lines). So a wave's 64 columns go through LDS, 16 rows at a time, and whole
-// lines go out; what is left behind a row's last line is carried to the next
-// pass. Only the ends of a block's columns are written in parts.
+// Lines of y that are written in two halves cost twice (2.1 GB of bf16 with
+// an odd number of words a row: 950 us, against 430 us for whole lines). So a
+// wave takes rows of x that lie the same way on lines, every `period`-th one,
+// and its columns begin on a line: `shift` columns before those of the tile
+// of w, out of this tile and the one before it. The block next to it ends
+// where this one begins.
 //
 // A wave's loads and stores are counted in one queue. The wait for a tile of
-// w therefore counts the stores after it, which are the same number in every
-// pass but a block's first and last: rows behind the last one repeat it.
-template <bool X4, bool OUT32, int R>
+// w therefore counts the stores behind it: they are the same number in every
+// pass but at the table's ends, because rows of x behind the last one repeat
+// it, and store the same again.
+template <bool X4, bool OUT32>
 struct Stream {
   static constexpr int XT = X4 ? 4 : 2;            // 16-row tiles of x a wave
   static constexpr int ES = OUT32 ? 4 : 2;
-  static constexpr int ROWS = 8 * XT * 16;         // rows of x a block
-  static constexpr int LINE = 128 / ES;
-  static constexpr int CROW = (LINE + 64) * ES + 16;   // carried columns, then new
-  static constexpr int RING = 64 * 4 * R * 17;     // codes, then scales
-  static constexpr int OWN = XT * 16 * 128 + 16 * CROW;
-  // tiles of w in LDS: as many as fit, four at most
-  static constexpr int DEPTH = (160 * 1024 - 8 * OWN) / RING >= 4   ? 4
-                               : (160 * 1024 - 8 * OWN) / RING >= 3 ? 3 : 2;
-  static constexpr int BYTES = DEPTH * RING + 8 * OWN;
-  static constexpr int STORES = XT * 16 * 64 * ES / 1024;   // a wave and pass
+  static constexpr int STORES = XT * 64 * ES / 64;          // a wave and pass
   static constexpr int LOADS = 3;                           // a wave and tile
+  static constexpr int ring_bytes(int r) { return 4 * 64 * 4 * r * 17; }
 };
 
 template <bool X4, bool OUT32, int R>
 __launch_bounds__(512, 2)
 __global__ void k_mxfp4_stream(MxArgs p) {
-  using S = Stream<X4, OUT32, R>;
-  constexpr int XT = S::XT, ES = S::ES, LINE = S::LINE, CROW = S::CROW, D = S::DEPTH;
-  extern __shared__ uint8_t sm[];
+  using S = Stream<X4, OUT32>;
+  constexpr int XT = S::XT, ES = S::ES;
+  extern __shared__ uint8_t sm[];              // 4 x 64 rows of codes, of scales
+  uint8_t* const sm_scales = sm + 4 * 64 * 4 * R * 16;
 
   const int b = xcd_chunked(blockIdx.x, gridDim.x);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, q = lane >> 4;
-  const int pass0 = b / p.n_tiles * p.passes_each;
-  const int pass1 = min(pass0 + p.passes_each, (p.M + 63) / 64);
-  if (pass0 >= pass1) return;
-  const int n0 = b % p.n_tiles * S::ROWS + wid * XT * 16;    // this wave's
-  uint8_t* carry = sm + D * S::RING + wid * S::OWN;          // (16 XT, LINE)
-  uint8_t* cbuf = carry + XT * 16 * 128;                     // (16, CROW)
-
-  // Rows of w lie in LDS in the order in which lanes take them: row 16t + i
-  // is row 16(i/4) + 4t + i%4 of the 64. A row's 16-byte blocks change places
-  // within groups of `group`, the power of two in their number, so that the
-  // 16 rows of a read lie on all banks.
   const int nb = p.nb;
-  const int group = min(nb & -nb, 16);
-  const int fold = __builtin_ctz(16 / group);
-  auto key = [&](int row) { return ((row & 15) >> fold) & (group - 1); };
-  auto fetch = [&](int pass) {
-    const int m0 = min(pass, pass1 - 1) * 64;
-    uint8_t* ring = sm + (pass % D) * S::RING;
+  const int pass0 = b / p.n_tiles * p.passes_each;
+  const int pass1 = min(pass0 + p.passes_each, p.passes);
+  if (pass0 >= pass1) return;
+
+  // this wave's rows: n0, n0 + period, ..; some waves have none
+  const int wave = b % p.n_tiles * 8 + wid;
+  const int first_n = wave % p.period + wave / p.period * (XT * 16) * p.period;
+  const bool idle = first_n >= p.N;
+  const int n0 = min(first_n, p.N - 1);
+  const int last = (p.N - 1 - n0) / p.period;
+  const int shift = p.period == 1 ? 0 :
+      (int)(((u64)p.y + (u64)n0 * p.M * ES) & 127) / ES;
+
+  // Four 16-byte blocks of a row change places by the row's number, where the
+  // number of blocks has the powers of two for it: a read's 16 rows then lie
+  // on more banks.
+  const int group = min(nb & -nb, 4);
+  auto key = [&](int row) { return (row >> 4) & (group - 1); };
+  auto fetch = [&](int tile) {        // rows 64 * tile ..
+    const int m0 = max(0, min(tile * 64, (p.M - 1) / 64 * 64));
     const uint8_t* wc = in_scalar(p.wc + (u64)m0 * nb * 16);
+    uint8_t* codes = sm + (tile & 3) * 64 * nb * 16;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       // 64 blocks an instruction, nb instructions a tile; a wave without one
       // repeats another
       const int e = wid + 8 * k < nb ? wid + 8 * k : wid % nb;
-      const int u = e * 64 + lane, j = u / nb, at = u % nb;
-      const int i = j & 15, row = (i >> 2) * 16 + (j >> 4) * 4 + (i & 3);
-      const u32 off = (u32)(min(row, p.M - 1 - m0) * nb + (at ^ key(j))) * 16;
-      to_lds<16>(wc + off, ring + e * 1024);
+      const int u = e * 64 + lane, row = u / nb, at = u % nb;
+      const u32 off = (u32)(min(row, p.M - 1 - m0) * nb + (at ^ key(row))) * 16;
+      to_lds<16>(wc + off, codes + e * 1024);
     }
     const int e = wid * 4 < nb ? wid : 0;
     const int whole = (min(64, p.M - m0) * nb) >> 2;       // words of scales
     // (a tile without a whole word: it is filled in below)
     const uint8_t* ws = in_scalar(p.ws + (whole ? (u64)m0 * nb : 0));
     to_lds<4>(ws + (u32)max(0, min(e * 64 + lane, whole - 1)) * 4,
-              ring + 64 * 4 * R * 16 + e * 256);
+              sm_scales + (tile & 3) * 256 * R + e * 256);
   };
 
   // x into registers; blocks behind a row's end are zeros
   u32x4 xf[XT][X4 ? R : R * 4];
   u32 xs[XT][R];
+  u32 y_off[XT];
 #pragma unroll
   for (int i = 0; i < XT; ++i) {
-    const int n = min(n0 + i * 16 + l16, p.N - 1);
+    const int j = min(i * 16 + l16, last);
+    const long n = n0 + (long)j * p.period;
+    y_off[i] = (u32)j * (u32)p.period * (u32)p.M * ES + q * 16 * ES;
 #pragma unroll
     for (int s = 0; s < R; ++s) {
       if constexpr (X4) {
         xf[i][s] = x_unit<true>(p, n, s * 4 + q, xs[i][s]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          xf[i][s * 4 + j] = x_unit<false>(p, n, (s * 4 + q) * 4 + j, xs[i][s]);
+        for (int j4 = 0; j4 < 4; ++j4)
+          xf[i][s * 4 + j4] = x_unit<false>(p, n, (s * 4 + q) * 4 + j4, xs[i][s]);
       }
     }
   }
-  for (int k = 0; k < D - 1; ++k) fetch(pass0 + k);
+  for (int k = -1; k < 2; ++k) fetch(pass0 + k);
 
-  // where this lane finds its block of step s in row l16 of a tile, and its
-  // scale; a step may have fewer than four blocks: the others repeat the last
-  u32 c_at[R], s_at[R];
-#pragma unroll
-  for (int s = 0; s < R; ++s) {
-    const int blk = min(s * 4 + q, nb - 1);
-    c_at[s] = (l16 * nb + (blk ^ key(l16))) * 16;
-    s_at[s] = 64 * 4 * R * 16 + ((l16 >> 2) * 16 + (l16 & 3)) * nb + blk;
-  }
+  // Row t*4 of this lane in a pass: behind the tile's first row, or in the
+  // tile before it. A step may have fewer than four blocks: the others repeat
+  // the last.
+  const int row_in = (l16 >> 2) * (4 * MT) + (l16 & 3) - shift;
+  const int left = nb - (R - 1) * 4;               // may be below one for R == 2
+  const int q_end = min(q, max(left, 1) - 1);
 
+  const int end = (p.M - 1) / 64;                  // the table's last tile
+  const int odd = (int)(((long)p.M * nb) & 3);
   f32x4 acc[XT][MT];
   for (int pass = pass0; pass < pass1; ++pass) {
-    const int m0 = pass * 64;
-    wait_queue<(D - 2) * S::LOADS, (D - 2) * S::LOADS + (D - 1) * S::STORES>(
-        pass - pass0 >= D);
-    const int odd = pass == (p.M - 1) / 64 ? (p.M - m0) * nb & 3 : 0;
-    if (odd) {
+    // behind this pass's tile: the next one, and the stores of two passes
+    const int m0 = pass * 64 - shift;
+    wait_queue<S::LOADS, S::LOADS + 2 * S::STORES>(
+        !idle && pass - pass0 >= 3 && m0 <= p.M);
+    if (odd && (pass == end || (pass == pass0 && pass == end + 1))) {
       // the table's last scales, where they fill no word
-      const int at = ((p.M - m0) * nb & ~3) + tid;
-      if (tid < odd)
-        sm[(pass % D) * S::RING + 64 * 4 * R * 16 + at] = p.ws[(u64)m0 * nb + at];
+      const int at = ((p.M - end * 64) * nb & ~3) + tid;
+      if (tid < odd) sm_scales[(end & 3) * 256 * R + at] = p.ws[(u64)end * 64 * nb + at];
       __syncthreads();
     }
-    fetch(pass + D - 1);
+    fetch(pass + 2);
     asm volatile("" ::: "memory");
-    const uint8_t* ring = sm + (pass % D) * S::RING;
+    if (idle) continue;
 
     mx_clear(acc);
+    const u32 now = (pass & 3) * 64, before = ((pass - 1) & 3) * 64;
 #pragma unroll
-    for (int s = 0; s < R; ++s) {
+    for (int t = 0; t < MT; ++t) {
+      const int row = row_in + t * 4;
+      const int in = row & 63;
+      const u32 at = row < 0 ? before : now;
+      const uint8_t* c_row = sm + (at + in) * nb * 16;
+      const uint8_t* s_row = sm_scales + at * 4 * R + in * nb;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const u32x4 c = *reinterpret_cast<const u32x4*>(ring + c_at[s] + t * 256 * nb);
-        u32 sc = ring[s_at[s] + t * 4 * nb];
-        sc = s * 4 + q < nb ? sc : 127;
+      for (int s = 0; s < R; ++s) {
+        if (R == 2 && s * 4 >= nb) break;
+        const int at_q = s == R - 1 ? q_end : q;
+        const u32x4 c = *reinterpret_cast<const u32x4*>(
+            c_row + s * 64 + (at_q ^ key(in)) * 16);
+        u32 sc = s_row[s * 4 + at_q];
+        if (s == R - 1 && q >= left) sc = 127;
         if constexpr (X4) {
           const i32x8 wf = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
 #pragma unroll
@@ -570,71 +579,39 @@ __global__ void k_mxfp4_stream(MxArgs p) {
     }
     mx_pin(acc);
 
-    // one 16-byte piece of a row a lane, RPI rows an instruction
-    constexpr int PER = 16 / ES, LPR = 64 / PER, RPI = 64 / LPR;
-    const bool first = pass == pass0, last = pass == pass1 - 1;
-    const int end = min(p.M - m0, 64);
-    int rl = lane / LPR;
-    // addresses are made here, not once for all passes: they would spill
-    asm volatile("" : "+v"(rl));
+    if (m0 >= 0 && m0 + 64 <= p.M) {
+      uint8_t* o = in_scalar(reinterpret_cast<uint8_t*>(p.y) +
+                             ((u64)n0 * p.M + m0) * ES);
 #pragma unroll
-    for (int i = 0; i < XT; ++i) {
-      uint8_t* mine = cbuf + l16 * CROW + (LINE + q * 16) * ES;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
+      for (int i = 0; i < XT; ++i) {
         if constexpr (OUT32) {
-          *reinterpret_cast<f32x4*>(mine + t * 16) = acc[i][t];
-        } else if (t % 2 == 0) {
-          *reinterpret_cast<u16x8*>(mine + t * 8) = pack8(acc[i][t], acc[i][t + 1]);
-        }
-      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<u32x4*>(cbuf + (h * 8 + (lane >> 3)) * CROW + (lane & 7) * 16) =
-            *reinterpret_cast<const u32x4*>(carry + i * 2048 + h * 1024 + lane * 16);
-#pragma unroll
-      for (int h = 0; h < 16; h += RPI) {
-        // column c of the pass is at row + (LINE + c) * ES; those below zero
-        // are carried from the pass before
-        const uint8_t* row = cbuf + (h + rl) * CROW;
-        const int n = min(n0 + i * 16 + h + rl, p.N - 1);
-        uint8_t* o = reinterpret_cast<uint8_t*>(p.y) + ((u64)n * p.M + m0) * ES;
-        const int tail = (int)((u64)o & 127) / ES;     // the same in all passes
-        const int c = lane % LPR * PER - tail;
-        if (!first && !last) {
-          *reinterpret_cast<u32x4*>(o + (long)c * ES) =
-              *reinterpret_cast<const u32x4_any*>(row + (LINE + c) * ES);
+          for (int t = 0; t < MT; ++t)
+            *reinterpret_cast<f32x4_any*>(o + y_off[i] + t * 16) = acc[i][t];
         } else {
-          if ((c >= 0 || !first) && c + PER <= end)
-            *reinterpret_cast<u32x4*>(o + (long)c * ES) =
-                *reinterpret_cast<const u32x4_any*>(row + (LINE + c) * ES);
-          // the ends of the block's columns, a lane a value
-          const int e = lane % LPR;
-          auto one = [&](int at) {
-            if constexpr (OUT32)
-              *reinterpret_cast<float*>(o + (long)at * 4) =
-                  *reinterpret_cast<const float*>(row + (LINE + at) * 4);
-            else
-              *reinterpret_cast<ushort*>(o + (long)at * 2) =
-                  *reinterpret_cast<const ushort*>(row + (LINE + at) * 2);
-          };
-          if (first && e < min((PER - tail % PER) % PER, end)) one(e);
-          if (last) {
-            // whole pieces of the last line, then what is left of it
-            const int c2 = 64 - tail + e * PER;
-            if (c2 + PER <= end)
-              *reinterpret_cast<u32x4*>(o + (long)c2 * ES) =
-                  *reinterpret_cast<const u32x4_any*>(row + (LINE + c2) * ES);
-            const int at = (end + tail) / PER * PER - tail + e;
-            if (e < PER && (at >= 0 || !first) && at < end) one(at);
-          }
+#pragma unroll
+          for (int t = 0; t < MT; t += 2)
+            *reinterpret_cast<u16x8_any*>(o + y_off[i] + t * 8) =
+                pack8(acc[i][t], acc[i][t + 1]);
         }
       }
+    } else {
+      // an end of the table
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<u32x4*>(carry + i * 2048 + h * 1024 + lane * 16) =
-            *reinterpret_cast<const u32x4*>(cbuf + (h * 8 + (lane >> 3)) * CROW +
-                                            64 * ES + (lane & 7) * 16);
+      for (int i = 0; i < XT; ++i) {
+        const long n = n0 + (long)min(i * 16 + l16, last) * p.period;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int m = m0 + q * 16 + t * 4 + r;
+            if (m < 0 || m >= p.M) continue;
+            if constexpr (OUT32)
+              reinterpret_cast<float*>(p.y)[n * p.M + m] = acc[i][t][r];
+            else
+              reinterpret_cast<__bf16*>(p.y)[n * p.M + m] = (__bf16)acc[i][t][r];
+          }
+      }
     }
   }
   // tiles of w that nobody needs may still be on their way into LDS
@@ -718,10 +695,10 @@ torch::Tensor mxfp4_dequantize(torch::Tensor codes, torch::Tensor scales,
 // How a launch's blocks share the work, `wanted` of them at a time.
 long share(MxArgs& a, int rows, int pass, int wanted) {
   a.n_tiles = (a.N + rows - 1) / rows;
-  const int passes = (a.M + pass - 1) / pass;
+  a.passes = (a.M + pass - 1) / pass;
   const int want = std::max(1, (wanted + a.n_tiles - 1) / a.n_tiles);
-  a.passes_each = (passes + want - 1) / want;
-  const long blocks = (long)a.n_tiles * ((passes + a.passes_each - 1) / a.passes_each);
+  a.passes_each = (a.passes + want - 1) / want;
+  const long blocks = (long)a.n_tiles * ((a.passes + a.passes_each - 1) / a.passes_each);
   TORCH_CHECK(blocks < (1L << 31), "too many tiles");
   return blocks;
 }
@@ -750,23 +727,34 @@ void launch_rows(MxArgs a) {
 
 template <bool X4, bool OUT32, int R>
 void launch_stream(const MxArgs& args) {
-  using S = Stream<X4, OUT32, R>;
-  static_assert(S::BYTES <= 160 * 1024, "LDS");
+  using S = Stream<X4, OUT32>;
+  constexpr int rows = S::XT * 16;              // a wave
   MxArgs a = args;
+  const int over = (int)((long)a.M * S::ES % 128);
+  a.period = 1;
+  for (int v = 128; over && v > 1 && over % v; v /= 2) a.period *= 2;
+  // Rows that lie alike have to fill a good part of a wave. (bf16 x, 512 rows
+  // by 261246, half a wave each: xx us; in order, on broken lines: xx us.)
+  if (a.N / a.period < rows / 2 || (long)rows * a.period * a.M * S::ES >= (1L << 32))
+    a.period = 1;
+  const int per = (a.N + a.period - 1) / a.period;
+  const long waves = (long)a.period * ((per + rows - 1) / rows);
   // one block a CU, 256 of them at a time
-  a.n_tiles = (a.N + S::ROWS - 1) / S::ROWS;
-  const int passes = (a.M + 63) / 64, slices = std::max(1, 256 / a.n_tiles);
-  a.passes_each = (passes + slices - 1) / slices;
-  const long blocks = (long)a.n_tiles * ((passes + a.passes_each - 1) / a.passes_each);
+  a.n_tiles = (int)((waves + 7) / 8);
+  a.passes = (a.M + (a.period > 1 ? 63 : 0) + 63) / 64;
+  const int slices = std::max(1, 256 / a.n_tiles);
+  a.passes_each = (a.passes + slices - 1) / slices;
+  const long blocks = (long)a.n_tiles * ((a.passes + a.passes_each - 1) / a.passes_each);
   TORCH_CHECK(blocks < (1L << 31), "too many tiles");
-  launch_mx(&k_mxfp4_stream<X4, OUT32, R>, a, blocks, 512, S::BYTES);
+  launch_mx(&k_mxfp4_stream<X4, OUT32, R>, a, blocks, 512, S::ring_bytes(R));
 }
 
 template <bool X4, bool OUT32>
 void pick_mx(const MxArgs& a) {
   const int steps = (a.nb + 3) / 4;
   if (a.N <= 16) launch_rows<X4, OUT32, 1>(a);
-  else if (a.N <= 128 || a.M < 64 || steps > 4) launch_rows<X4, OUT32, 4>(a);
+  else if (a.N <= 128 || a.M < 64 || steps > 4 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
+    launch_rows<X4, OUT32, 4>(a);
   else if (steps <= 2) launch_stream<X4, OUT32, 2>(a);
   else if (steps == 3) launch_stream<X4, OUT32, 3>(a);
   else launch_stream<X4, OUT32, 4>(a);

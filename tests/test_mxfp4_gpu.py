@@ -116,7 +116,8 @@ def on_gpu(q):
     (1, 1000, 384), (1, 1, 1), (3, 7, 5), (16, 512, 128), (17, 513, 32), (15, 511, 384),
     (37, 501, 201), (64, 700, 96), (65, 1030, 160), (130, 520, 384), (200, 77, 640),
     (40, 300, 1030), (5, 200, 2500), (129, 1500, 385), (300, 4100, 384), (513, 5003, 33),
-    (260, 9001, 100), (700, 3000, 511), (1030, 2050, 384)])
+    (260, 9001, 100), (700, 3000, 511), (1030, 2050, 384), (2100, 1501, 64),
+    (530, 70, 300), (600, 64, 40), (140, 129, 7)])
 def test_products(N, M, K, out):
     x = rows(N, K, N, BF) * 0.5
     w = R.mxfp4_quantize(rows(M, K, M + 1))
