@@ -124,6 +124,65 @@ struct BtArgs {
   const long* seed_ptr;
 };
 
+// GT f32x4 of a lane, consecutive columns from h of a row of H: 16-byte stores
+// (8 for GT = 1) where rows lie on them
+template <int GT>
+DEVI void put(ushort* base, const float* v, int h, int H) {
+  constexpr int W = GT == 1 ? 4 : 8;
+  if (H % W == 0) {
+#pragma unroll
+    for (int c = 0; c < 4 * GT; c += W)
+      if (h + c < H) {
+        if constexpr (GT == 1) {
+          bf16x4 b;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = (__bf16)v[j];
+          *reinterpret_cast<bf16x4*>(base) = b;
+        } else {
+          *reinterpret_cast<u16x8*>(base + c) = pack8(v + c);
+        }
+      }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4 * GT; ++c)
+      if (h + c < H) base[c] = __builtin_bit_cast(ushort, (__bf16)v[c]);
+  }
+}
+
+template <int ACT, int GT>
+DEVI void put_gated(const BtArgs& p, long n, int h, const f32x4* g, const f32x4* u) {
+  float gv[4 * GT], uv[4 * GT], yv[4 * GT];
+#pragma unroll
+  for (int j = 0; j < 4 * GT; ++j) {
+    gv[j] = g[j / 4][j & 3];
+    uv[j] = u[j / 4][j & 3];
+    float a, da;
+    act_both<ACT>(gv[j], a, da);
+    yv[j] = a * uv[j];
+  }
+  put<GT>(p.y + n * p.H + h, yv, h, p.H);
+  if (p.gu) {
+    put<GT>(p.gu + n * 2 * p.Hp + h, gv, h, p.H);
+    put<GT>(p.gu + n * 2 * p.Hp + p.Hp + h, uv, h, p.H);
+  }
+}
+
+template <int GT>
+DEVI void put_plain(const BtArgs& p, long n, int h, const f32x4* a) {
+  float v[4 * GT];
+#pragma unroll
+  for (int j = 0; j < 4 * GT; ++j) v[j] = a[j / 4][j & 3];
+  if (p.keep_prob < 1.f) {
+    const u64 seed = p.seed_ptr ? (u64)*p.seed_ptr : p.seed;
+    const float inv_keep = 1.f / p.keep_prob;
+#pragma unroll
+    for (int j = 0; j < 4 * GT; ++j)
+      v[j] = hash_uniform(seed, (u64)n * p.H + h + j) < p.keep_prob ? v[j] * inv_keep
+                                                                   : 0.f;
+  }
+  put<GT>(p.y + n * p.H + h, v, h, p.H);
+}
+
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK,
           int STAGES>
 __launch_bounds__(WR * WC * 64, 2)
@@ -233,65 +292,98 @@ __global__ void k_rows_gemm(BtArgs p) {
     }
   }
 
-  const bool vec = (p.H & 7) == 0;
-  const u64 seed = p.seed_ptr ? (u64)*p.seed_ptr : p.seed;
-  const float inv_keep = 1.f / p.keep_prob;
-  // run = values of one lane in one group, consecutive columns from h
-  auto put = [&](ushort* base, const float* v, int h) {
-#pragma unroll
-    for (int c = 0; c < 4 * GT; c += 4) {
-      if (vec && GT >= 2) {
-        if (c % 8 == 0 && h + c < p.H)
-          *reinterpret_cast<u16x8*>(base + c) = pack8(v + c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (h + c + j < p.H)
-            base[c + j] = __builtin_bit_cast(ushort, (__bf16)v[c + j]);
-      }
-    }
-  };
 #pragma unroll
   for (int i = 0; i < XT; ++i) {
     const long n = row0 + wr * XT * 16 + i * 16 + l16;
     if (n >= p.N) continue;
     if constexpr (EPI == GATED) {
-      const int h = h0 + wc * GT * 16 + q * 4 * GT;
-      float gv[4 * GT], uv[4 * GT], yv[4 * GT];
-#pragma unroll
-      for (int j = 0; j < GT; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          gv[j * 4 + r] = acc[i][j][r];
-          uv[j * 4 + r] = acc[i][GT + j][r];
-          float a, da;
-          act_both<ACT>(gv[j * 4 + r], a, da);
-          yv[j * 4 + r] = a * uv[j * 4 + r];
-        }
-      put(p.y + n * p.H + h, yv, h);
-      if (p.gu) {
-        put(p.gu + n * 2 * p.Hp + h, gv, h);
-        put(p.gu + n * 2 * p.Hp + p.Hp + h, uv, h);
-      }
+      put_gated<ACT, GT>(p, n, h0 + wc * GT * 16 + q * 4 * GT, acc[i], acc[i] + GT);
     } else {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int h = h0 + (wc * 2 + g) * GT * 16 + q * 4 * GT;
-        float v[4 * GT];
-#pragma unroll
-        for (int j = 0; j < GT; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float t = acc[i][g * GT + j][r];
-            if (p.keep_prob < 1.f) {
-              const u64 e = (u64)n * p.H + h + j * 4 + r;
-              t = hash_uniform(seed, e) < p.keep_prob ? t * inv_keep : 0.f;
-            }
-            v[j * 4 + r] = t;
-          }
-        put(p.y + n * p.H + h, v, h);
-      }
+      put_plain<GT>(p, n, h0 + wc * 2 * GT * 16 + q * 4 * GT, acc[i]);
+      put_plain<GT>(p, n, h0 + (wc * 2 + 1) * GT * 16 + q * 4 * GT, acc[i] + GT);
     }
+  }
+}
+
+// The same for few rows of x. Bound by reading w, and by how long that takes
+// one after the other: a block's four waves share 16 columns (of gate and up;
+// 32 of a plain product) and cut the reduction, step by step in turn; their
+// sums are added in order in LDS. Operands go from memory to registers, two
+// steps ahead.
+template <int EPI, int ACT, int XT>
+__launch_bounds__(256)
+__global__ void k_rows_skinny(BtArgs p) {
+  constexpr int HT = EPI == GATED ? 16 : 32;
+  __shared__ f32x4 sums[4][XT][2][64];
+  const int nC = (p.H + HT - 1) / HT;
+  const int wg = xcd_chunked(blockIdx.x, gridDim.x);
+  const long row0 = (long)(wg / nC) * XT * 16;
+  const int h0 = (wg % nC) * HT;
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, q = lane >> 4;
+
+  const ushort *x[XT], *w[2];
+#pragma unroll
+  for (int i = 0; i < XT; ++i)
+    x[i] = p.x + min(row0 + i * 16 + l16, (long)p.N - 1) * p.ldx;
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    w[g] = p.w + (EPI == GATED ? (long)g * p.H + min(h0 + l16, p.H - 1)
+                               : (long)min(h0 + g * 16 + l16, p.H - 1)) * p.K;
+  struct Step { bf16x8 x[XT], w[2]; };
+  auto load = [&](int s) {
+    const int k = s * 32 + q * 8;
+    Step v;
+#pragma unroll
+    for (int i = 0; i < XT; ++i)
+      v.x[i] = *reinterpret_cast<const bf16x8*>(k < p.K ? x[i] + k : k_zero_chunk);
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+      v.w[g] = *reinterpret_cast<const bf16x8*>(k < p.K ? w[g] + k : k_zero_chunk);
+    return v;
+  };
+  f32x4 acc[XT][2];
+#pragma unroll
+  for (int i = 0; i < XT; ++i)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) acc[i][g] = {0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const Step& v) {
+#pragma unroll
+    for (int i = 0; i < XT; ++i)
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        acc[i][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v.w[g], v.x[i], acc[i][g],
+                                                            0, 0, 0);
+  };
+  // beyond the end the chunks are zeros, and add nothing
+  Step a = load(wid), b = load(wid + 4);
+  const int steps = (p.K + 31) / 32;
+  for (int s = wid; s < steps; s += 8) {
+    const Step c = load(s + 8), d = load(s + 12);
+    step(a);
+    step(b);
+    a = c;
+    b = d;
+  }
+#pragma unroll
+  for (int i = 0; i < XT; ++i)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) sums[wid][i][g][lane] = acc[i][g];
+  __syncthreads();
+  if (wid >= XT) return;
+  const long n = row0 + wid * 16 + l16;
+  if (n >= p.N) return;
+  f32x4 v[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    v[g] = sums[0][wid][g][lane] + sums[1][wid][g][lane] + sums[2][wid][g][lane] +
+           sums[3][wid][g][lane];
+  if constexpr (EPI == GATED) {
+    put_gated<ACT, 1>(p, n, h0 + q * 4, v, v + 1);
+  } else {
+    put_plain<1>(p, n, h0 + q * 4, v);
+    put_plain<1>(p, n, h0 + 16 + q * 4, v + 1);
   }
 }
 
@@ -353,12 +445,17 @@ __global__ void k_gated_dgu(const ushort* __restrict__ gu,
 
 constexpr int TN_ROWS = 32;
 
+// where the 16-column unit `unit` of row r lies, in rows of `cols` columns
+DEVI int dw_place(int unit, int r, int cols) {
+  return unit ^ (r & 7 & (cols / 16 - 1));
+}
+
 DEVI bf16x8 tr_read(const ushort* tile, int stride, int c0, int l16, int q) {
   s16x4 v[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = half * 16 + q * 4 + (l16 >> 2);
-    const int unit = (c0 >> 4) ^ (r & 7);
+    const int unit = dw_place(c0 >> 4, r, stride);
     const ushort* a = tile + r * stride + unit * 16 + (l16 & 3) * 4;
     v[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
         (__attribute__((address_space(3))) s16x4*)a);
@@ -372,8 +469,9 @@ template <int WA, int WB, int AT, int BT>
 __launch_bounds__(WA * WB * 64, 2)
 __global__ void k_dw_part(const ushort* __restrict__ dgu,
                           const ushort* __restrict__ x, long ldx,
-                          float* __restrict__ part, int N, int C2, int K,
-                          int K8, int rows_each, int tiles) {
+                          float* __restrict__ part, ushort* __restrict__ d_w,
+                          int N, int C2, int K, int K8, int H, int rows_each,
+                          int tiles) {
   constexpr int T = WA * WB * 64;
   constexpr int CA = WA * AT * 16;     // columns of dgu a block
   constexpr int CB = WB * BT * 16;     // columns of x a block
@@ -404,7 +502,7 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
     const int c = (ina ? it : it - ITA) * T + tid;
     const int per = (ina ? CA : CB) / 8;
     const int r = c / per, pos = c % per;
-    const int cc = (((pos >> 1) ^ (r & 7)) * 2 + (pos & 1)) * 8;
+    const int cc = (dw_place(pos >> 1, r, ina ? CA : CB) * 2 + (pos & 1)) * 8;
     off[it] = ina ? (u32)((long)r * C2 + (a0 + cc < C2 ? a0 + cc : 0)) * 2
                   : (u32)((long)r * ldx + (b0 + cc < K8 ? b0 + cc : 0)) * 2;
   }
@@ -462,7 +560,8 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[i], bf[j],
                                                             acc[i][j], 0, 0, 0);
   }
-  // part (S, K, C2): a lane holds four consecutive columns of C2
+  // part (S, K, C2), or d_w itself if the rows are one part: a lane holds four
+  // consecutive columns of C2
 #pragma unroll
   for (int j = 0; j < BT; ++j) {
     const int k = b0 + (wb * BT + j) * 16 + l16;
@@ -470,9 +569,14 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
       const int c = a0 + (wa * AT + i) * 16 + q * 4;
-      if (c < C2)
-        *reinterpret_cast<f32x4*>(part + ((long)slice * K + k) * C2 + c) =
-            acc[i][j];
+      if (c >= C2) continue;
+      if (part) {
+        *reinterpret_cast<f32x4*>(part + ((long)slice * K + k) * C2 + c) = acc[i][j];
+      } else {
+        const int g = c >= C2 / 2, h = c - g * (C2 / 2);
+        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        put<1>(d_w + ((long)g * K + k) * H + h, v, h, H);
+      }
     }
   }
 }
@@ -590,24 +694,98 @@ void launch_rows(const BtArgs& a) {
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-template <int EPI, int ACT>
-void rows_gemm(const BtArgs& a) {
-  launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a);
+template <int EPI, int ACT, int XT>
+void launch_skinny(const BtArgs& a) {
+  constexpr int HT = EPI == GATED ? 16 : 32;
+  const long tiles = ((long)a.N + XT * 16 - 1) / (XT * 16) * ((a.H + HT - 1) / HT);
+  TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
+  auto* fn = &k_rows_skinny<EPI, ACT, XT>;
+  fn<<<(int)tiles, 256, 0, cur_stream()>>>(a);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-// How many parts the rows are cut into for dW. 512 blocks run at a time: a
-// part more than fills them costs a whole round, and every part costs the
+// What a launch takes, in us: `slots` blocks run at a time; a step takes one
+// of them `alone` in an idle chip and `full` in a full one.
+double launch_us(double blocks, double slots, double steps, double alone,
+                 double full, double fixed) {
+  const double load = std::min(1.0, blocks / slots);
+  return std::max(1.0, blocks / slots) * (fixed + steps * (alone + (full - alone) * load));
+}
+
+// Tiles from 256 rows by 128 columns of gate and up down to 16 by 16: large
+// ones read least, small ones fill the chip. The rates are fitted to both
+// products at 1..204800 rows and widths of 96..1440; what they choose is
+// within a tenth of the best of these at three sizes of four. In us, by tile:
+//   rows  width   256x128   128x64   64x32   32x16
+//    200    384      14.7      6.9     4.5     4.0
+//   1024    768      24.3     11.3     8.1    19.3
+//   4096   1440      45.2     49.3    84.5   201
+// 204800    384       214      245     359    906
+template <int EPI, int ACT>
+void rows_gemm(const BtArgs& a) {
+  constexpr double plain = EPI == PLAIN ? 2 : 1;    // groups of columns a tile
+  auto blocks = [&](double rows, double cols) {
+    return std::ceil(a.N / rows) * std::ceil(a.H / (cols * plain));
+  };
+  const double k64 = (a.K + 63) / 64, k32 = (a.K + 31) / 32;
+  const double us[] = {
+      launch_us(blocks(256, 128), 256, k64, 1.25, 2.2, 5.0),
+      launch_us(blocks(128, 64), 512, k64, 0.60, 1.25, 3.0),
+      launch_us(blocks(64, 32), 768, k64, 0.30, 0.85, 2.0),
+      launch_us(blocks(a.N <= 16 ? 16 : 32, 16), 1024, k32, 0.045, 0.36, 2.6)};
+  switch (std::min_element(us, us + 4) - us) {
+    case 0: return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a);
+    case 1: return launch_rows<EPI, ACT, 2, 2, 4, 2, 64, 2>(a);
+    case 2: return launch_rows<EPI, ACT, 2, 2, 2, 1, 64, 3>(a);
+    default:
+      if (a.N <= 16) launch_skinny<EPI, ACT, 1>(a);
+      else launch_skinny<EPI, ACT, 2>(a);
+  }
+}
+
+// dW by tiles of CA columns of dgu by CB of x, the rows in S parts. A part
+// more than fills the chip costs a whole round, and every part costs the
 // writing and reading of its sums.
-int dw_parts(long tiles, long N, long outputs) {
-  int best = 1;
-  double least = 1e30;
-  for (long S = 1; S <= 64 && (S == 1 || N / S >= 256); ++S) {
-    const long rounds = (tiles * S + 511) / 512;
-    const double rows = (double)rounds * (N / S + 96);     // one block's, and its start
-    const double us = rows * 0.030 + (double)S * outputs * 8 / 5e6;
-    if (us < least) { least = us; best = (int)S; }
+struct DwPlan { double us; int S; };
+
+DwPlan plan_dw(long N, long C2, long K, int CA, int CB, double slots, double alone,
+               double full) {
+  const double tiles = std::ceil(C2 / (double)CA) * std::ceil(K / (double)CB);
+  DwPlan best{1e30, 1};
+  for (int S = 1; S <= 64 && (S == 1 || N / S >= 64); ++S) {
+    const double load = std::min(1.0, tiles * S / slots);
+    const double us = std::ceil(tiles * S / slots) *
+                          (3 + std::ceil(N / (double)S / TN_ROWS) * (alone + (full - alone) * load)) +
+                      (S > 1 ? 3 + S * (double)(C2 * K) * 8 / 5e6 : 0);
+    if (us < best.us) best = {us, S};
   }
   return best;
+}
+
+template <int WA, int WB, int AT, int BT>
+void launch_dw(const torch::Tensor& d_w, const ushort* dgu, const Rows& x, long N,
+               int K, int H, int Hp, int S) {
+  constexpr int CA = WA * AT * 16, CB = WB * BT * 16;
+  constexpr size_t bytes = 3ul * TN_ROWS * (CA + CB) * sizeof(ushort);
+  const int tiles = (2 * Hp + CA - 1) / CA * ((K + CB - 1) / CB);
+  const int rows_each = (int)(((N + S - 1) / S + TN_ROWS - 1) / TN_ROWS * TN_ROWS);
+  torch::Tensor part;
+  if (S > 1)
+    part = torch::empty({S, K, 2L * Hp}, d_w.options().dtype(torch::kFloat32));
+  auto* fn = &k_dw_part<WA, WB, AT, BT>;
+  if (bytes > 64 * 1024)
+    C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)bytes));
+  fn<<<tiles * S, WA * WB * 64, bytes, cur_stream()>>>(
+      dgu, x.p, x.ld, S > 1 ? part.data_ptr<float>() : nullptr, bf_mut(d_w), (int)N,
+      2 * Hp, K, pad8(K), H, rows_each, tiles);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
+  if (S == 1) return;
+  const long quads = (long)K * 2 * Hp / 4;
+  k_dw_reduce<<<(int)((quads + 255) / 256), 256, 0, cur_stream()>>>(
+      part.data_ptr<float>(), bf_mut(d_w), S, K, H, Hp);
+  C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
 template <int ACT>
@@ -703,25 +881,13 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   rows_gemm<PLAIN, SILU>(a);
 
   const Rows x = chunked_rows(ctx, K);
-  constexpr int WA = 2, WB = 2, AT = 8, BT = 4;
-  const int tiles = (2 * Hp + WA * AT * 16 - 1) / (WA * AT * 16) *
-                    ((K + WB * BT * 16 - 1) / (WB * BT * 16));
-  const int S = dw_parts(tiles, N, (long)K * 2 * Hp);
-  const int rows_each = (int)((((long)N + S - 1) / S + TN_ROWS - 1) / TN_ROWS * TN_ROWS);
-  auto part = torch::empty({S, K, 2L * Hp}, ctx.options().dtype(torch::kFloat32));
-  constexpr size_t bytes = 3ul * TN_ROWS * (WA * AT + WB * BT) * 16 * sizeof(ushort);
-  auto* dw = &k_dw_part<WA, WB, AT, BT>;
-  C10_HIP_CHECK(hipFuncSetAttribute(
-      (const void*)dw, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  dw<<<tiles * S, WA * WB * 64, bytes, cur_stream()>>>(
-      bf_ptr(dgu), x.p, x.ld, part.data_ptr<float>(), N, 2 * Hp, K, pad8(K),
-      rows_each, tiles);
-  C10_HIP_KERNEL_LAUNCH_CHECK();
   auto d_w = torch::empty({2, K, H}, ctx.options());
-  const long quads = (long)K * 2 * Hp / 4;
-  k_dw_reduce<<<(int)((quads + 255) / 256), 256, 0, cur_stream()>>>(
-      part.data_ptr<float>(), bf_mut(d_w), S, K, H, Hp);
-  C10_HIP_KERNEL_LAUNCH_CHECK();
+  const DwPlan large = plan_dw(N, 2L * Hp, K, 256, 128, 512, 0.6, 1.3);
+  const DwPlan small = plan_dw(N, 2L * Hp, K, 64, 64, 1024, 0.3, 0.6);
+  if (large.us <= small.us)
+    launch_dw<2, 2, 8, 4>(d_w, bf_ptr(dgu), x, N, K, H, Hp, large.S);
+  else
+    launch_dw<2, 2, 2, 2>(d_w, bf_ptr(dgu), x, N, K, H, Hp, small.S);
   return {d_ctx, d_w};
 }
 
