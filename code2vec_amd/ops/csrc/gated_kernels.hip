@@ -834,7 +834,7 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
                                                torch::Tensor gu,
                                                torch::Tensor d_y, int64_t act,
                                                double keep_prob, int64_t seed,
-                                               torch::Tensor seed_t) {
+                                               c10::optional<torch::Tensor> seed_t) {
   check_bf16(ctx, "ctx", 2, ctx);
   check_bf16(w_io, "w_io", 2, ctx);
   check_bf16(gu, "gu", 3, ctx);
@@ -848,11 +848,11 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
               gu.is_contiguous(), "gu must be what the forward kept");
   TORCH_CHECK(keep_prob > 0.0 && keep_prob <= 1.0, "keep_prob must be in (0, 1]");
   const long* seed_ptr = nullptr;
-  if (seed_t.defined() && seed_t.numel() == 1) {
-    TORCH_CHECK(seed_t.device() == ctx.device() &&
-                seed_t.scalar_type() == torch::kInt64,
+  if (seed_t) {
+    TORCH_CHECK(seed_t->numel() == 1 && seed_t->device() == ctx.device() &&
+                seed_t->scalar_type() == torch::kInt64,
                 "seed_t must be one int64 on the GPU that ctx is on");
-    seed_ptr = seed_t.data_ptr<long>();
+    seed_ptr = seed_t->data_ptr<long>();
   }
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
   auto d_ctx = torch::empty({N, K}, ctx.options());

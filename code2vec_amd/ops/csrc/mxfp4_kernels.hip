@@ -760,20 +760,21 @@ void pick_mx(const MxArgs& a) {
   else launch_stream<X4, OUT32, 4>(a);
 }
 
-// x: bf16 (N, K) with x_scales empty, or the codes of x and their scales
-torch::Tensor mxfp4_matmul(torch::Tensor x, torch::Tensor x_scales,
+// x: bf16 (N, K), or the codes of x with their scales
+torch::Tensor mxfp4_matmul(torch::Tensor x,
+                           c10::optional<torch::Tensor> x_scales,
                            torch::Tensor w_codes, torch::Tensor w_scales,
                            int64_t K, bool f32) {
   check_mx(w_codes, w_scales, K, "w");
-  const bool x4 = x.scalar_type() == torch::kUInt8;
+  const bool x4 = x_scales.has_value();
   TORCH_CHECK(x.device() == w_codes.device(), "x and w must be on one GPU");
   const Guard guard(x.device());
   torch::Tensor src = x;
   MxArgs a{};
   if (x4) {
-    check_mx(x, x_scales, K, "x");
+    check_mx(x, *x_scales, K, "x");
     a.xc = x.data_ptr<uint8_t>();
-    a.xs = x_scales.data_ptr<uint8_t>();
+    a.xs = x_scales->data_ptr<uint8_t>();
   } else {
     TORCH_CHECK(x.scalar_type() == torch::kBFloat16 && x.dim() == 2 &&
                 x.size(1) == K, "x must be a bfloat16 (N, K)");

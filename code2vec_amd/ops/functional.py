@@ -65,9 +65,8 @@ def transform_tanh_bwd(ctx, w_io_bf16, y, d_y) -> Tuple[torch.Tensor, torch.Tens
     return d_ctx, d_w
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise ValueError(what)
+def _refuse(what: str, *values):
+    raise ValueError(what % values)
 
 
 def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
@@ -80,14 +79,14 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
     gu): gu holds what transform_gated_bwd needs if `save`, else None. On the
     GPU all are bfloat16 (sums and activation in fp32), any N, K and H; rows
     of ctx may be any stride apart."""
-    _need(activation in GATE_ACTIVATIONS, 'activation must be one of %s, not %r'
-          % (', '.join(GATE_ACTIVATIONS), activation))
-    _need(ctx.dim() == 2 and w_oi.dim() == 3 and w_oi.shape[0] == 2
-          and w_oi.shape[2] == ctx.shape[1],
-          'ctx (N,K) and w_oi (2,H,K) do not fit: %s and %s'
-          % (tuple(ctx.shape), tuple(w_oi.shape)))
-    _need(ctx.dtype == w_oi.dtype and ctx.device == w_oi.device,
-          'ctx and w_oi must have one type and one device')
+    if activation not in GATE_ACTIVATIONS:
+        _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
+    if (ctx.dim() != 2 or w_oi.dim() != 3 or w_oi.shape[0] != 2
+            or w_oi.shape[2] != ctx.shape[1]):
+        _refuse('ctx (N,K) and w_oi (2,H,K) do not fit: %s and %s',
+                tuple(ctx.shape), tuple(w_oi.shape))
+    if ctx.dtype != w_oi.dtype or ctx.device != w_oi.device:
+        _refuse('ctx and w_oi must have one type and one device')
     if backend_for(ctx) == 'hip':
         y, gu = hip_ext(True).transform_gated_fwd(
             ctx, w_oi, GATE_ACTIVATIONS.index(activation), bool(save))
@@ -103,24 +102,25 @@ def transform_gated_bwd(ctx, w_io, gu, d_y, activation: str = 'silu',
     forward kept; d_y (N,H). Returns (d_ctx (N,K), d_w (2,K,H)), in ctx's
     type. With keep_prob < 1 d_ctx goes through the keep mask of the dropout
     that made ctx (gather_concat_fwd with the same seed) on its way out."""
-    _need(activation in GATE_ACTIVATIONS, 'activation must be one of %s, not %r'
-          % (', '.join(GATE_ACTIVATIONS), activation))
-    _need(ctx.dim() == 2 and d_y.dim() == 2 and d_y.shape[0] == ctx.shape[0]
-          and tuple(w_io.shape) == (ctx.shape[1], 2 * d_y.shape[1]),
-          'ctx (N,K), w_io (K,2H) and d_y (N,H) do not fit: %s, %s and %s'
-          % (tuple(ctx.shape), tuple(w_io.shape), tuple(d_y.shape)))
-    _need(gu is not None, 'the forward kept nothing: call it with save=True')
-    _need(tuple(gu.shape) == (ctx.shape[0], 2, -(-d_y.shape[1] // 8) * 8),
-          'gu is not what the forward of this ctx kept')
-    _need(all(t.dtype == ctx.dtype and t.device == ctx.device
-              for t in (w_io, gu, d_y)),
-          'ctx, w_io, gu and d_y must have one type and one device')
-    _need(0.0 < keep_prob <= 1.0, 'keep_prob must be in (0, 1]')
+    if activation not in GATE_ACTIVATIONS:
+        _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
+    if (ctx.dim() != 2 or d_y.dim() != 2 or d_y.shape[0] != ctx.shape[0]
+            or w_io.shape != (ctx.shape[1], 2 * d_y.shape[1])):
+        _refuse('ctx (N,K), w_io (K,2H) and d_y (N,H) do not fit: %s, %s and %s',
+                tuple(ctx.shape), tuple(w_io.shape), tuple(d_y.shape))
+    if gu is None:
+        _refuse('the forward kept nothing: call it with save=True')
+    if gu.shape != (ctx.shape[0], 2, -(-d_y.shape[1] // 8) * 8):
+        _refuse('gu is not what the forward of this ctx kept')
+    for t in (w_io, gu, d_y):
+        if t.dtype != ctx.dtype or t.device != ctx.device:
+            _refuse('ctx, w_io, gu and d_y must have one type and one device')
+    if not 0.0 < keep_prob <= 1.0:
+        _refuse('keep_prob must be in (0, 1]')
     if backend_for(ctx) == 'hip':
         d_ctx, d_w = hip_ext(True).transform_gated_bwd(
-            ctx, w_io, gu, d_y, GATE_ACTIVATIONS.index(activation),
-            float(keep_prob), int(seed),
-            seed_t if seed_t is not None else torch.empty(0))
+            ctx, w_io, gu, d_y, GATE_ACTIVATIONS.index(activation), keep_prob,
+            seed, seed_t)
         return d_ctx, d_w
     d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, gu, d_y, activation)
     if keep_prob < 1.0:
@@ -131,18 +131,18 @@ def transform_gated_bwd(ctx, w_io, gu, d_y, activation: str = 'silu',
 
 
 def _check_mxfp4(q, name: str):
-    _need(isinstance(q, Mxfp4), '%s must be an Mxfp4' % name)
+    if not isinstance(q, Mxfp4):
+        _refuse('%s must be an Mxfp4', name)
     blocks = -(-q.k // ref.MXFP4_BLOCK)
-    _need(q.codes.dtype == torch.uint8 and q.scales.dtype == torch.uint8,
-          '%s must hold uint8 codes and scales' % name)
-    _need(q.codes.dim() == 2 and q.scales.dim() == 2
-          and q.codes.shape[0] == q.scales.shape[0]
-          and q.scales.shape[1] == blocks and q.codes.shape[1] == 16 * blocks,
-          '%s does not hold rows of %d values: codes %s, scales %s'
-          % (name, q.k, tuple(q.codes.shape), tuple(q.scales.shape)))
-    _need(q.codes.is_contiguous() and q.scales.is_contiguous()
-          and q.codes.device == q.scales.device,
-          '%s must be contiguous and on one device' % name)
+    if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8:
+        _refuse('%s must hold uint8 codes and scales', name)
+    rows = q.scales.shape[0] if q.scales.dim() else 0
+    if q.codes.shape != (rows, 16 * blocks) or q.scales.shape != (rows, blocks):
+        _refuse('%s does not hold rows of %d values: codes %s, scales %s', name, q.k,
+                tuple(q.codes.shape), tuple(q.scales.shape))
+    if (not q.codes.is_contiguous() or not q.scales.is_contiguous()
+            or q.codes.device != q.scales.device):
+        _refuse('%s must be contiguous and on one device', name)
 
 
 def mxfp4_quantize(x) -> Mxfp4:
@@ -150,9 +150,10 @@ def mxfp4_quantize(x) -> Mxfp4:
     a row under one power of two, each value a 4-bit float (e2m1), rounded to
     nearest even and saturating. A block that holds a NaN or an infinity
     becomes NaN. Any N and K, rows any stride apart."""
-    _need(x.dim() == 2, 'x must be (N,K), not %s' % (tuple(x.shape),))
-    _need(x.dtype in (torch.float32, torch.bfloat16),
-          'x must be float32 or bfloat16, not %s' % x.dtype)
+    if x.dim() != 2:
+        _refuse('x must be (N,K), not %s', (tuple(x.shape),))
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        _refuse('x must be float32 or bfloat16, not %s', x.dtype)
     if backend_for(x) == 'hip':
         codes, scales = hip_ext(True).mxfp4_quantize(x)
         return Mxfp4(codes, scales, x.shape[1])
@@ -163,8 +164,8 @@ def mxfp4_dequantize(q: Mxfp4, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, (N,K). They are exact in either dtype,
     bfloat16 or float32."""
     _check_mxfp4(q, 'q')
-    _need(dtype in (torch.float32, torch.bfloat16),
-          'dtype must be float32 or bfloat16, not %s' % dtype)
+    if dtype not in (torch.float32, torch.bfloat16):
+        _refuse('dtype must be float32 or bfloat16, not %s', dtype)
     if backend_for(q.codes) == 'hip':
         return hip_ext(True).mxfp4_dequantize(q.codes, q.scales, q.k,
                                               dtype == torch.float32)
@@ -180,22 +181,23 @@ def mxfp4_matmul(x, w: Mxfp4, out_dtype=torch.bfloat16) -> torch.Tensor:
     into the scaled matrix instructions as they are. Any N, M and K. There is
     no backward: this is what a trained table answers with."""
     _check_mxfp4(w, 'w')
-    _need(out_dtype in (torch.float32, torch.bfloat16),
-          'out_dtype must be float32 or bfloat16, not %s' % out_dtype)
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        _refuse('out_dtype must be float32 or bfloat16, not %s', out_dtype)
+    scales = None
     if isinstance(x, Mxfp4):
         _check_mxfp4(x, 'x')
-        _need(x.k == w.k, 'x has rows of %d values, w of %d' % (x.k, w.k))
-        _need(x.codes.device == w.codes.device, 'x and w must be on one device')
-        if backend_for(w.codes) == 'hip':
-            return hip_ext(True).mxfp4_matmul(x.codes, x.scales, w.codes, w.scales,
-                                              w.k, out_dtype == torch.float32)
-        return ref.mxfp4_matmul(x, w, out_dtype)
-    _need(x.dim() == 2 and x.shape[1] == w.k,
-          'x must be (N,%d), not %s' % (w.k, tuple(x.shape)))
-    _need(x.device == w.codes.device, 'x and w must be on one device')
+        if x.k != w.k:
+            _refuse('x has rows of %d values, w of %d', x.k, w.k)
+        rows, scales = x.codes, x.scales
+    else:
+        if x.dim() != 2 or x.shape[1] != w.k:
+            _refuse('x must be (N,%d), not %s', w.k, tuple(x.shape))
+        rows = x
+    if rows.device != w.codes.device:
+        _refuse('x and w must be on one device')
     if backend_for(w.codes) == 'hip':
-        return hip_ext(True).mxfp4_matmul(x, torch.empty(0), w.codes, w.scales,
-                                          w.k, out_dtype == torch.float32)
+        return hip_ext(True).mxfp4_matmul(rows, scales, w.codes, w.scales, w.k,
+                                          out_dtype == torch.float32)
     return ref.mxfp4_matmul(x, w, out_dtype)
 
 
