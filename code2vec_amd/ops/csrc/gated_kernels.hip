@@ -94,18 +94,20 @@ DEVI u16x8 pack8(const float* v) {
 // product.
 // ---------------------------------------------------------------------------
 
-// Tiles go from memory into a ring of LDS buffers, STAGES - 1 steps ahead of
+// Tiles go from memory into a ring of LDS buffers, one or two steps ahead of
 // the matrix instructions. A step begins when its own tile has arrived, which
-// is when no more than the `younger` loads issued after it are outstanding,
-// and when every wave has read the tile that the step's new loads overwrite.
-template <int PER_TILE, int STAGES>
-DEVI void wait_tile(int left) {   // left: steps after this one
-  static_assert(PER_TILE < 64 && (STAGES == 2 || STAGES == 3), "vmcnt has 6 bits");
+// is when no more than N of the loads and stores that this wave issued after
+// it are outstanding, and when every wave has read the tile that the step's
+// new loads overwrite.
+template <int N>
+DEVI void wait_queue() {
+  static_assert(N < 64, "vmcnt has 6 bits");
   // vmcnt in bits 3:0 and 15:14, expcnt 6:4 (no wait), lgkmcnt 11:8 (zero)
-  constexpr int none = 0x70, one = 0x70 | (PER_TILE & 15) | (PER_TILE >> 4 << 14);
   asm volatile("" ::: "memory");
-  if (STAGES == 3 && left > 0) __builtin_amdgcn_s_waitcnt(one);
-  else __builtin_amdgcn_s_waitcnt(none);
+  __builtin_amdgcn_s_waitcnt(0x70 | (N & 15) | (N >> 4 << 14));
+}
+
+DEVI void block_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -200,10 +202,15 @@ __global__ void k_rows_gemm(BtArgs p) {
   static_assert(BM * CH % T == 0 && BN * CH % T == 0, "staging");
   extern __shared__ ushort lds[];          // STAGES x (BM + BN) x BK
 
+  // An XCD's blocks go over a run of tiles together, those of one tile of x
+  // next to each other: its rows come from one L2.
   const int nC = (p.H + HT - 1) / HT;
-  const int wg = xcd_chunked(blockIdx.x, gridDim.x);
-  const long row0 = (long)(wg / nC) * BM;
-  const int h0 = (wg % nC) * HT;
+  const int tiles = (int)((p.N + (long)BM - 1) / BM * nC);
+  const int xcd = blockIdx.x & 7, each = (gridDim.x + 7 - xcd) >> 3;
+  const int tile0 = xcd * (tiles >> 3) + min(xcd, tiles & 7);
+  const int tile1 = tile0 + (tiles >> 3) + (xcd < (tiles & 7));
+  int tile = tile0 + (blockIdx.x >> 3);
+  if (tile >= tile1) return;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -212,30 +219,40 @@ __global__ void k_rows_gemm(BtArgs p) {
 
   // Where each of this thread's chunks comes from: bytes behind the tile's
   // first row of x, or behind w. A step adds to the bases alone.
+  long row0;
+  int h0;
   u32 off[IT];
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int c = it * T + tid;
-    const int r = c / CH, pos = c % CH;
-    const u32 col = (pos ^ place(r)) * 16;
-    if (it < ITX) {
-      const long n = min((long)r, (long)p.N - 1 - row0);
-      off[it] = (u32)(n * p.ldx * 2) + col;
-    } else {
-      const int j = r - BM;                       // row of w in LDS
-      const int i = j & 15, mi = (j >> 4) % GT;
-      const int grp = (j >> 4) / GT % 2, cw = (j >> 4) / (2 * GT);
-      const int in_group = (i >> 2) * (4 * GT) + mi * 4 + (i & 3);
-      long wrow;
-      if constexpr (EPI == GATED)
-        wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
-      else
-        wrow = min(h0 + (cw * 2 + grp) * GT * 16 + in_group, p.H - 1);
-      off[it] = (u32)(wrow * p.K * 2) + col;
-    }
-  }
-  const char* xb = reinterpret_cast<const char*>(p.x + row0 * p.ldx);
+  const char* xb;
   const char* wb = reinterpret_cast<const char*>(p.w);
+  auto begin = [&](int t) {
+    row0 = (long)(t / nC) * BM;
+    h0 = t % nC * HT;
+    xb = reinterpret_cast<const char*>(p.x + row0 * p.ldx);
+    // made here for each tile: kept over the tiles its parts would spill
+    int me = tid;
+    asm volatile("" : "+v"(me));
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      const int c = it * T + me;
+      const int r = c / CH, pos = c % CH;
+      const u32 col = (pos ^ place(r)) * 16;
+      if (it < ITX) {
+        const long n = min((long)r, (long)p.N - 1 - row0);
+        off[it] = (u32)(n * p.ldx * 2) + col;
+      } else {
+        const int j = r - BM;                       // row of w in LDS
+        const int i = j & 15, mi = (j >> 4) % GT;
+        const int grp = (j >> 4) / GT % 2, cw = (j >> 4) / (2 * GT);
+        const int in_group = (i >> 2) * (4 * GT) + mi * 4 + (i & 3);
+        long wrow;
+        if constexpr (EPI == GATED)
+          wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
+        else
+          wrow = min(h0 + (cw * 2 + grp) * GT * 16 + in_group, p.H - 1);
+        off[it] = (u32)(wrow * p.K * 2) + col;
+      }
+    }
+  };
   auto stage = [&](int k0, int buf) {
     ushort* dst = lds + buf * (BM + BN) * BK + wid * 512;
     if (k0 + BK <= p.K) {
@@ -255,53 +272,78 @@ __global__ void k_rows_gemm(BtArgs p) {
     }
   };
 
-  f32x4 acc[XT][2 * GT];
-#pragma unroll
-  for (int i = 0; i < XT; ++i)
-#pragma unroll
-    for (int j = 0; j < 2 * GT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
-
+  // stores of a wave in a tile's end, where all of it is there
+  constexpr int PUT = XT * (GT >= 2 ? GT / 2 : 1);
   const int steps = (p.K + BK - 1) / BK;
+  bool whole = false;                      // the tile before was
+  int buf = 0;
+  begin(tile);
   stage(0, 0);
   if (STAGES == 3 && steps > 1) stage(BK, 1);
-  int buf = 0;
-  for (int s = 0; s < steps; ++s) {
-    wait_tile<IT, STAGES>(steps - 1 - s);
-    if (s + STAGES - 1 < steps)
-      stage((s + STAGES - 1) * BK, buf == 0 ? STAGES - 1 : buf - 1);
-    const ushort* xs = lds + buf * (BM + BN) * BK + wr * XT * 16 * BK;
-    const ushort* ws = lds + buf * (BM + BN) * BK +
-                       (BM + wc * 2 * GT * 16) * BK;
-    buf = buf == STAGES - 1 ? 0 : buf + 1;
+  for (;;) {
+    f32x4 acc[XT][2 * GT];
 #pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      const int off = l16 * BK + (((kk * 4 + q) ^ place(l16)) * 8);
-      bf16x8 xf[XT], wf[2 * GT];
+    for (int i = 0; i < XT; ++i)
 #pragma unroll
-      for (int i = 0; i < XT; ++i)
-        xf[i] = *reinterpret_cast<const bf16x8*>(xs + i * 16 * BK + off);
+      for (int j = 0; j < 2 * GT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+    long row = row0;
+    int h = h0;
+    const bool more = STAGES == 2 && tile + each < tile1;
+    for (int s = 0; s < steps; ++s) {
+      if (STAGES == 3 ? s + 1 < steps : false) {
+        wait_queue<IT>();
+      } else if (STAGES == 2 && s == 0 && whole) {
+        // the stores of the tile before are behind this tile's loads
+        if (EPI == PLAIN) wait_queue<2 * PUT>();
+        else if (p.gu) wait_queue<3 * PUT>();
+        else wait_queue<PUT>();
+      } else {
+        wait_queue<0>();
+      }
+      block_barrier();
+      const int into = STAGES == 2 ? buf ^ 1 : buf == 0 ? 2 : buf - 1;
+      if (s + STAGES - 1 < steps) {
+        stage((s + STAGES - 1) * BK, into);
+      } else if (more) {
+        begin(tile + each);
+        stage(0, into);
+      }
+      const ushort* xs = lds + buf * (BM + BN) * BK + wr * XT * 16 * BK;
+      const ushort* ws = lds + buf * (BM + BN) * BK +
+                         (BM + wc * 2 * GT * 16) * BK;
+      buf = buf == STAGES - 1 ? 0 : buf + 1;
 #pragma unroll
-      for (int j = 0; j < 2 * GT; ++j)
-        wf[j] = *reinterpret_cast<const bf16x8*>(ws + j * 16 * BK + off);
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        const int off = l16 * BK + (((kk * 4 + q) ^ place(l16)) * 8);
+        bf16x8 xf[XT], wf[2 * GT];
 #pragma unroll
-      for (int i = 0; i < XT; ++i)
+        for (int i = 0; i < XT; ++i)
+          xf[i] = *reinterpret_cast<const bf16x8*>(xs + i * 16 * BK + off);
 #pragma unroll
         for (int j = 0; j < 2 * GT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              wf[j], xf[i], acc[i][j], 0, 0, 0);
-    }
-  }
-
+          wf[j] = *reinterpret_cast<const bf16x8*>(ws + j * 16 * BK + off);
 #pragma unroll
-  for (int i = 0; i < XT; ++i) {
-    const long n = row0 + wr * XT * 16 + i * 16 + l16;
-    if (n >= p.N) continue;
-    if constexpr (EPI == GATED) {
-      put_gated<ACT, GT>(p, n, h0 + wc * GT * 16 + q * 4 * GT, acc[i], acc[i] + GT);
-    } else {
-      put_plain<GT>(p, n, h0 + wc * 2 * GT * 16 + q * 4 * GT, acc[i]);
-      put_plain<GT>(p, n, h0 + (wc * 2 + 1) * GT * 16 + q * 4 * GT, acc[i] + GT);
+        for (int i = 0; i < XT; ++i)
+#pragma unroll
+          for (int j = 0; j < 2 * GT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                wf[j], xf[i], acc[i][j], 0, 0, 0);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < XT; ++i) {
+      const long n = row + wr * XT * 16 + i * 16 + l16;
+      if (n >= p.N) continue;
+      if constexpr (EPI == GATED) {
+        put_gated<ACT, GT>(p, n, h + wc * GT * 16 + q * 4 * GT, acc[i], acc[i] + GT);
+      } else {
+        put_plain<GT>(p, n, h + wc * 2 * GT * 16 + q * 4 * GT, acc[i]);
+        put_plain<GT>(p, n, h + (wc * 2 + 1) * GT * 16 + q * 4 * GT, acc[i] + GT);
+      }
+    }
+    if (!more) return;
+    whole = row + BM <= p.N && h + HT <= p.H && p.H % (GT == 1 ? 4 : 8) == 0;
+    tile += each;
   }
 }
 
@@ -540,7 +582,9 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
   if (steps > 1) stage(n0 + TN_ROWS, 1);
   int buf = 0;
   for (int s = 0; s < steps; ++s) {
-    wait_tile<ITA + ITB, 3>(steps - 1 - s);
+    if (s + 1 < steps) wait_queue<ITA + ITB>();
+    else wait_queue<0>();
+    block_barrier();
     if (s + 2 < steps)
       stage(n0 + (long)(s + 2) * TN_ROWS, buf == 0 ? 2 : buf - 1);
     const ushort* la = lds + buf * BUF;
@@ -678,8 +722,9 @@ Rows chunked_rows(const torch::Tensor& t, int cols) {
   return {out, bf_ptr(out), (long)pad8(cols)};
 }
 
+// `slots` blocks at a time, each over several tiles
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK, int STAGES>
-void launch_rows(const BtArgs& a) {
+void launch_rows(const BtArgs& a, long slots) {
   constexpr int BM = WR * XT * 16, BG = WC * GT * 16;
   constexpr int HT = EPI == GATED ? BG : 2 * BG;
   constexpr size_t bytes = (size_t)STAGES * (BM + 2 * BG) * BK * sizeof(ushort);
@@ -690,7 +735,8 @@ void launch_rows(const BtArgs& a) {
                                        (int)bytes));
   const long tiles = ((long)a.N + BM - 1) / BM * ((a.H + HT - 1) / HT);
   TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
-  fn<<<(int)tiles, WR * WC * 64, bytes, cur_stream()>>>(a);
+  fn<<<(int)std::min(tiles, STAGES == 2 ? slots : tiles), WR * WC * 64, bytes,
+       cur_stream()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
@@ -734,9 +780,9 @@ void rows_gemm(const BtArgs& a) {
       launch_us(blocks(64, 32), 768, k64, 0.30, 0.85, 2.0),
       launch_us(blocks(a.N <= 16 ? 16 : 32, 16), 1024, k32, 0.045, 0.36, 2.6)};
   switch (std::min_element(us, us + 4) - us) {
-    case 0: return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a);
-    case 1: return launch_rows<EPI, ACT, 2, 2, 4, 2, 64, 2>(a);
-    case 2: return launch_rows<EPI, ACT, 2, 2, 2, 1, 64, 3>(a);
+    case 0: return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a, 256);
+    case 1: return launch_rows<EPI, ACT, 2, 2, 4, 2, 64, 2>(a, 512);
+    case 2: return launch_rows<EPI, ACT, 2, 2, 2, 1, 64, 3>(a, 768);
     default:
       if (a.N <= 16) launch_skinny<EPI, ACT, 1>(a);
       else launch_skinny<EPI, ACT, 2>(a);
