@@ -37,8 +37,9 @@ def build(verbose: bool = True) -> str:
     os.makedirs(build_dir, exist_ok=True)
     sources = _hip_sources(here)
     dest = os.path.join(here, '_c2v_hip.so')
-    if _is_fresh(dest, *sources, os.path.join(here, 'csrc', 'c2v_device.h'),
-                 os.path.abspath(__file__)):
+    headers = [os.path.join(here, 'csrc', name)
+               for name in ('c2v_device.h', 'c2v_launch.h')]
+    if _is_fresh(dest, *sources, *headers, os.path.abspath(__file__)):
         build_reader(verbose=verbose)
         return dest
 

@@ -15,6 +15,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 
 #include "c2v_device.h"
+#include "c2v_launch.h"
 
 namespace {
 
@@ -667,15 +668,7 @@ __global__ void k_pad_cols(const ushort* __restrict__ in, long ld,
 // host wrappers
 // ===========================================================================
 
-inline hipStream_t cur_stream() {
-  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-}
-
 inline int pad8(int v) { return (v + 7) / 8 * 8; }
-
-inline int grid_of(long items, int block, long cap) {
-  return (int)std::max(1L, std::min((items + block - 1) / block, cap));
-}
 
 const ushort* bf_ptr(const torch::Tensor& t) {
   return reinterpret_cast<const ushort*>(t.data_ptr<at::BFloat16>());
@@ -729,10 +722,8 @@ void launch_rows(const BtArgs& a, long slots) {
   constexpr int HT = EPI == GATED ? BG : 2 * BG;
   constexpr size_t bytes = (size_t)STAGES * (BM + 2 * BG) * BK * sizeof(ushort);
   auto* fn = &k_rows_gemm<EPI, ACT, WR, WC, XT, GT, BK, STAGES>;
-  if (bytes > 64 * 1024)
-    C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
-                                       hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)bytes));
+  static std::atomic<u64> ready{0};
+  allow_lds(fn, bytes, ready);
   const long tiles = ((long)a.N + BM - 1) / BM * ((a.H + HT - 1) / HT);
   TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
   fn<<<(int)std::min(tiles, STAGES == 2 ? slots : tiles), WR * WC * 64, bytes,
@@ -755,7 +746,7 @@ void launch_skinny(const BtArgs& a) {
 double launch_us(double blocks, double slots, double steps, double alone,
                  double full, double fixed) {
   const double load = std::min(1.0, blocks / slots);
-  return std::max(1.0, blocks / slots) * (fixed + steps * (alone + (full - alone) * load));
+  return std::ceil(blocks / slots) * (fixed + steps * (alone + (full - alone) * load));
 }
 
 // Tiles from 256 rows by 128 columns of gate and up down to 16 by 16: large
@@ -819,10 +810,8 @@ void launch_dw(const torch::Tensor& d_w, const ushort* dgu, const Rows& x, long 
   if (S > 1)
     part = torch::empty({S, K, 2L * Hp}, d_w.options().dtype(torch::kFloat32));
   auto* fn = &k_dw_part<WA, WB, AT, BT>;
-  if (bytes > 64 * 1024)
-    C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
-                                      hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)bytes));
+  static std::atomic<u64> ready{0};
+  allow_lds(fn, bytes, ready);
   fn<<<tiles * S, WA * WB * 64, bytes, cur_stream()>>>(
       dgu, x.p, x.ld, S > 1 ? part.data_ptr<float>() : nullptr, bf_mut(d_w), (int)N,
       2 * Hp, K, pad8(K), H, rows_each, tiles);

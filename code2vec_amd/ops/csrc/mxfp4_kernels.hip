@@ -15,13 +15,13 @@
 #include <type_traits>
 
 #include "c2v_device.h"
+#include "c2v_launch.h"
 
 namespace {
 
 // vectors at any address of their element's type
 using u16x8_any = u16x8 __attribute__((aligned(2)));
 using f32x4_any = f32x4 __attribute__((aligned(4)));
-using u32x4_any = u32x4 __attribute__((aligned(2)));
 
 DEVI float scale_of(u32 byte) {
   // what the conversion instructions read of a scale is its exponent field,
@@ -97,36 +97,39 @@ __launch_bounds__(256)
 __global__ void k_mxfp4_quantize(const void* __restrict__ x, long ldx,
                                  u32* __restrict__ codes,
                                  uint8_t* __restrict__ scales, long R, int K,
-                                 int nb, int vec) {
+                                 int nb, int vec, int flat) {
   const long per_row = (long)nb * 4, total = R * per_row;
   // whole wavefronts stay in the loop together: the shuffles need all lanes
   for (long base = (long)blockIdx.x * 256; base < total;
        base += (long)gridDim.x * 256) {
     const long t = base + threadIdx.x;
-    const long r = t / per_row;
-    const int k = (int)(t - r * per_row) * 8;
+    // (a division of 32 bits is a third of one of 64)
+    const long r = flat ? 0 : total <= 0xFFFFFFFFl ? (long)((u32)t / (u32)per_row)
+                                                   : t / per_row;
+    const long k = (t - r * per_row) * 8;
+    const long K_ = flat ? R * K : K;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (t < total) {
       if constexpr (F32) {
         const float* p = reinterpret_cast<const float*>(x) + r * ldx + k;
-        if (vec && k + 8 <= K) {
+        if (vec && k + 8 <= K_) {
           const f32x4 a = *reinterpret_cast<const f32x4*>(p);
           const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) if (k + j < K) v[j] = p[j];
+          for (int j = 0; j < 8; ++j) if (k + j < K_) v[j] = p[j];
         }
       } else {
         const ushort* p = reinterpret_cast<const ushort*>(x) + r * ldx + k;
-        if (vec && k + 8 <= K) {
+        if (vec && k + 8 <= K_) {
           const u16x8 a = *reinterpret_cast<const u16x8*>(p);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = bf2f(a[j]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) if (k + j < K) v[j] = bf2f(p[j]);
+          for (int j = 0; j < 8; ++j) if (k + j < K_) v[j] = bf2f(p[j]);
         }
       }
     }
@@ -160,10 +163,13 @@ __global__ void k_mxfp4_dequantize(const u32* __restrict__ codes,
                                    int nb) {
   const int per_row = (K + 7) / 8;
   const long total = R * per_row;
+  const bool flat = K % 32 == 0;
   for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total;
        t += (long)gridDim.x * 256) {
-    const long r = t / per_row;
-    const int c8 = (int)(t - r * per_row), k = c8 * 8;
+    const long r = flat ? 0 : total <= 0xFFFFFFFFl ? (long)((u32)t / (u32)per_row)
+                                                   : t / per_row;
+    const long c8 = t - r * per_row, k = c8 * 8;
+    const long K_ = flat ? R * K : K;
     const bf16x8 v = decode8(codes[r * nb * 4 + c8],
                              scale_of(scales[r * nb + (c8 >> 2)]));
     if constexpr (F32) {
@@ -171,21 +177,21 @@ __global__ void k_mxfp4_dequantize(const u32* __restrict__ codes,
       f32x4 a, b;
 #pragma unroll
       for (int j = 0; j < 4; ++j) { a[j] = (float)v[j]; b[j] = (float)v[4 + j]; }
-      if (k + 8 <= K) {
+      if (k + 8 <= K_) {
         *reinterpret_cast<f32x4_any*>(o) = a;
         *reinterpret_cast<f32x4_any*>(o + 4) = b;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (k + j < K) o[j] = (float)v[j];
+        for (int j = 0; j < 8; ++j) if (k + j < K_) o[j] = (float)v[j];
       }
     } else {
       ushort* o = reinterpret_cast<ushort*>(out) + r * K + k;
       const u16x8 a = __builtin_bit_cast(u16x8, v);
-      if (k + 8 <= K) {
+      if (k + 8 <= K_) {
         *reinterpret_cast<u16x8_any*>(o) = a;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (k + j < K) o[j] = a[j];
+        for (int j = 0; j < 8; ++j) if (k + j < K_) o[j] = a[j];
       }
     }
   }
@@ -431,19 +437,20 @@ __global__ void k_mxfp4_rows(MxArgs p) {
 // w therefore counts the stores behind it: they are the same number in every
 // pass but at the table's ends, because rows of x behind the last one repeat
 // it, and store the same again.
-template <bool X4, bool OUT32>
+template <bool X4, bool OUT32, int R>
 struct Stream {
-  static constexpr int XT = X4 ? 4 : 2;            // 16-row tiles of x a wave
+  static constexpr int XT = X4 ? 4 : R > 4 ? 1 : 2;   // 16-row tiles of x a wave
   static constexpr int ES = OUT32 ? 4 : 2;
   static constexpr int STORES = XT * 64 * ES / 64;          // a wave and pass
-  static constexpr int LOADS = 3;                           // a wave and tile
-  static constexpr int ring_bytes(int r) { return 4 * 64 * 4 * r * 17; }
+  static constexpr int FETCH = (4 * R + 7) / 8;             // of them codes
+  static constexpr int LOADS = FETCH + 1;                   // a wave and tile
+  static constexpr int RING = 4 * 64 * 4 * R * 17;
 };
 
 template <bool X4, bool OUT32, int R>
 __launch_bounds__(512, 2)
 __global__ void k_mxfp4_stream(MxArgs p) {
-  using S = Stream<X4, OUT32>;
+  using S = Stream<X4, OUT32, R>;
   constexpr int XT = S::XT, ES = S::ES;
   extern __shared__ uint8_t sm[];              // 4 x 64 rows of codes, of scales
   uint8_t* const sm_scales = sm + 4 * 64 * 4 * R * 16;
@@ -476,7 +483,7 @@ __global__ void k_mxfp4_stream(MxArgs p) {
     const uint8_t* wc = in_scalar(p.wc + (u64)m0 * nb * 16);
     uint8_t* codes = sm + (tile & 3) * 64 * nb * 16;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < S::FETCH; ++k) {
       // 64 blocks an instruction, nb instructions a tile; a wave without one
       // repeats another
       const int e = wid + 8 * k < nb ? wid + 8 * k : wid % nb;
@@ -622,14 +629,6 @@ __global__ void k_mxfp4_stream(MxArgs p) {
 // host wrappers
 // ===========================================================================
 
-inline hipStream_t cur_stream() {
-  return at::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-}
-
-inline int grid_of(long items, int block, long cap) {
-  return (int)std::max(1L, std::min((items + block - 1) / block, cap));
-}
-
 using Guard = c10::hip::OptionalHIPGuardMasqueradingAsCUDA;
 
 std::vector<torch::Tensor> mxfp4_quantize(torch::Tensor x) {
@@ -648,11 +647,13 @@ std::vector<torch::Tensor> mxfp4_quantize(torch::Tensor x) {
   const long ld = R == 1 ? K : src.stride(0);
   const int vec = (ld % (f32 ? 4 : 8)) == 0 &&
                   (reinterpret_cast<uintptr_t>(src.data_ptr()) & 15) == 0;
+  // dense rows of whole blocks are one long row: no division is needed
+  const int flat = K % 32 == 0 && (ld == K || R == 1);
   const int grid = grid_of(R * nb * 4, 256, 16384);
   auto* fn = f32 ? &k_mxfp4_quantize<true> : &k_mxfp4_quantize<false>;
   fn<<<grid, 256, 0, cur_stream()>>>(
       src.data_ptr(), ld, reinterpret_cast<u32*>(codes.data_ptr()),
-      scales.data_ptr<uint8_t>(), R, K, nb, vec);
+      scales.data_ptr<uint8_t>(), R, K, nb, vec, flat);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {codes, scales};
 }
@@ -703,12 +704,11 @@ long share(MxArgs& a, int rows, int pass, int wanted) {
   return blocks;
 }
 
-template <typename Fn>
-void launch_mx(Fn* fn, const MxArgs& a, long blocks, int threads, size_t bytes) {
-  if (bytes > 64 * 1024)
-    C10_HIP_CHECK(hipFuncSetAttribute((const void*)fn,
-                                      hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)bytes));
+template <void (*KERNEL)(MxArgs)>
+void launch_mx(const MxArgs& a, long blocks, int threads, size_t bytes) {
+  static std::atomic<u64> ready{0};
+  auto* fn = KERNEL;
+  allow_lds(fn, 160 * 1024, ready);
   fn<<<(int)blocks, threads, bytes, cur_stream()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
@@ -722,20 +722,28 @@ void launch_rows(MxArgs a) {
   a.kc = std::min((a.nb * 32 + 127) / 128 * 128, most);
   const size_t bytes = (size_t)ROWS * ((X4 ? a.kc / 2 : a.kc * 2) + 16) +
                        (X4 ? (size_t)ROWS * (a.kc / 32) : 0);
-  launch_mx(&k_mxfp4_rows<X4, OUT32, XT>, a, blocks, 256, bytes);
+  launch_mx<&k_mxfp4_rows<X4, OUT32, XT>>(a, blocks, 256, bytes);
 }
 
 template <bool X4, bool OUT32, int R>
 void launch_stream(const MxArgs& args) {
-  using S = Stream<X4, OUT32>;
+  using S = Stream<X4, OUT32, R>;
   constexpr int rows = S::XT * 16;              // a wave
   MxArgs a = args;
   const int over = (int)((long)a.M * S::ES % 128);
   a.period = 1;
   for (int v = 128; over && v > 1 && over % v; v /= 2) a.period *= 2;
-  // Rows that lie alike have to fill a good part of a wave. (bf16 x, 512 rows
-  // by 261246, half a wave each: xx us; in order, on broken lines: xx us.)
-  if (a.N / a.period < rows / 2 || (long)rows * a.period * a.M * S::ES >= (1L << 32))
+  // In order a wave writes broken lines. The cache behind L2 mends them as long
+  // as y is not much larger than it, and rows that lie alike have to fill their
+  // waves. (M = 261246, K = 384, bf16 y; rows alike against in order: bf16 x, 512
+  // rows in half-filled waves 208 us to 118, 1024 in full ones 217 to 249; 4-bit
+  // x 512 rows in a quarter 150 to 92, 768 in 3/8 172 to 215, 4096 518 to 1142.
+  // M = 50001, 4-bit x: 1024 rows, 102 MB, 60 to 46; 4096, 410 MB, 117 to 228.)
+  const long alike = (a.N + a.period - 1) / a.period;
+  const long held = (alike + rows - 1) / rows * rows;
+  if ((long)a.N * a.M * S::ES < (192L << 20) ||
+      (X4 ? 8 * alike < 3 * held : 4 * alike <= 3 * held) ||
+      (long)rows * a.period * a.M * S::ES >= (1L << 32))
     a.period = 1;
   const int per = (a.N + a.period - 1) / a.period;
   const long waves = (long)a.period * ((per + rows - 1) / rows);
@@ -746,18 +754,20 @@ void launch_stream(const MxArgs& args) {
   a.passes_each = (a.passes + slices - 1) / slices;
   const long blocks = (long)a.n_tiles * ((a.passes + a.passes_each - 1) / a.passes_each);
   TORCH_CHECK(blocks < (1L << 31), "too many tiles");
-  launch_mx(&k_mxfp4_stream<X4, OUT32, R>, a, blocks, 512, S::ring_bytes(R));
+  launch_mx<&k_mxfp4_stream<X4, OUT32, R>>(a, blocks, 512, S::RING);
 }
 
 template <bool X4, bool OUT32>
 void pick_mx(const MxArgs& a) {
   const int steps = (a.nb + 3) / 4;
   if (a.N <= 16) launch_rows<X4, OUT32, 1>(a);
-  else if (a.N <= 128 || a.M < 64 || steps > 4 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
+  else if (a.N <= 128 || a.M < 64 || steps > 6 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
     launch_rows<X4, OUT32, 4>(a);
   else if (steps <= 2) launch_stream<X4, OUT32, 2>(a);
   else if (steps == 3) launch_stream<X4, OUT32, 3>(a);
-  else launch_stream<X4, OUT32, 4>(a);
+  else if (steps == 4) launch_stream<X4, OUT32, 4>(a);
+  else if (steps == 5) launch_stream<X4, OUT32, 5>(a);
+  else launch_stream<X4, OUT32, 6>(a);
 }
 
 // x: bf16 (N, K), or the codes of x with their scales

@@ -117,7 +117,8 @@ def on_gpu(q):
     (37, 501, 201), (64, 700, 96), (65, 1030, 160), (130, 520, 384), (200, 77, 640),
     (40, 300, 1030), (5, 200, 2500), (129, 1500, 385), (300, 4100, 384), (513, 5003, 33),
     (260, 9001, 100), (700, 3000, 511), (1030, 2050, 384), (2100, 1501, 64),
-    (530, 70, 300), (600, 64, 40), (140, 129, 7)])
+    (530, 70, 300), (600, 64, 40), (140, 129, 7), (257, 1027, 545), (600, 3002, 768),
+    (130, 500, 641), (200, 300, 769)])
 def test_products(N, M, K, out):
     x = rows(N, K, N, BF) * 0.5
     w = R.mxfp4_quantize(rows(M, K, M + 1))
@@ -137,6 +138,19 @@ def test_whole_numbers_are_exact():
     assert torch.equal(F.mxfp4_dequantize(wq, F32).cpu(), w)
     assert torch.equal(F.mxfp4_matmul(x.to(BF).cuda(), wq, F32).cpu(), x @ w.t())
     assert torch.equal(F.mxfp4_matmul(F.mxfp4_quantize(x.cuda()), wq, F32).cpu(), x @ w.t())
+
+
+@pytest.mark.parametrize('N,M,K,out', [(2040, 50001, 70, BF), (1000, 50003, 300, F32),
+                                       (2048, 50004, 130, BF), (4000, 25002, 40, BF)])
+def test_more_than_the_caches_hold(N, M, K, out):
+    """Whole numbers again, so that each result is exact up to its own rounding."""
+    g = torch.Generator(device='cuda').manual_seed(1)
+    x = torch.randint(-4, 5, (N, K), generator=g, device='cuda').float()
+    w = torch.randint(-4, 5, (M, K), generator=g, device='cuda').float()
+    want = (x @ w.t()).to(out)
+    wq = F.mxfp4_quantize(w)
+    assert torch.equal(F.mxfp4_matmul(x.to(BF), wq, out), want)
+    assert torch.equal(F.mxfp4_matmul(F.mxfp4_quantize(x), wq, out), want)
 
 
 @pytest.mark.parametrize('N', [5, 100])
