@@ -17,6 +17,10 @@ from typing import Optional
 class Config:
     """All knobs in one object, passed to every layer (reference: config.py:9)."""
 
+    TRANSFORMS = ('tanh', 'gated')
+    GATE_ACTIVATIONS = ('silu', 'gelu', 'sigmoid', 'relu', 'tanh')
+    TARGET_FORMATS = ('full', 'w4', 'w4a4')
+
     @classmethod
     def arguments_parser(cls) -> ArgumentParser:
         # Same CLI surface as the reference (config.py:11-44), minus the
@@ -74,6 +78,18 @@ class Config:
                             type=int, default=0,
                             help="if >0, train with sampled softmax over this many negatives "
                                  "(evaluation always uses the full softmax)")
+        parser.add_argument('--transform', dest='transform', default='tanh',
+                            choices=list(cls.TRANSFORMS),
+                            help="what combines a context's three vectors: one projection "
+                                 "and tanh, or a gated pair of projections")
+        parser.add_argument('--gate-activation', dest='gate_activation', default='silu',
+                            choices=list(cls.GATE_ACTIVATIONS),
+                            help="activation of the gate (with --transform gated)")
+        parser.add_argument('--target-format', dest='target_format', default='full',
+                            choices=list(cls.TARGET_FORMATS),
+                            help="what evaluation and prediction score names with: the target "
+                                 "table in the compute dtype, its MXFP4 codes (w4), or "
+                                 "those and MXFP4 code vectors (w4a4)")
         return parser
 
     def set_defaults(self):
@@ -107,6 +123,9 @@ class Config:
         self.DEVICE = None              # resolved lazily; 'cuda' is ROCm/HIP on this stack
         self.COMPUTE_DTYPE = 'bf16'     # GEMMs in bf16 (MFMA), masters fp32
         self.SAMPLED_SOFTMAX_SIZE = 0   # 0 = full softmax (reference behavior)
+        self.TRANSFORM = 'tanh'         # 'gated': act(ctx Wg) * (ctx Wu)
+        self.GATE_ACTIVATION = 'silu'
+        self.TARGET_FORMAT = 'full'     # 'w4', 'w4a4': answers from MXFP4 codes
         self.ADAM_LR = 0.001            # TF AdamOptimizer defaults (reference K10)
         self.ADAM_BETA1 = 0.9
         self.ADAM_BETA2 = 0.999
@@ -133,6 +152,9 @@ class Config:
         self.DEVICE = args.device
         self.COMPUTE_DTYPE = args.compute_dtype
         self.SAMPLED_SOFTMAX_SIZE = args.sampled_softmax_size
+        self.TRANSFORM = args.transform
+        self.GATE_ACTIVATION = args.gate_activation
+        self.TARGET_FORMAT = args.target_format
 
     def __init__(self, set_defaults: bool = False, load_from_args: bool = False,
                  verify: bool = False):
@@ -178,6 +200,9 @@ class Config:
         self.DEVICE: Optional[str] = None
         self.COMPUTE_DTYPE: str = 'bf16'
         self.SAMPLED_SOFTMAX_SIZE: int = 0
+        self.TRANSFORM: str = 'tanh'
+        self.GATE_ACTIVATION: str = 'silu'
+        self.TARGET_FORMAT: str = 'full'
         self.ADAM_LR: float = 0.001
         self.ADAM_BETA1: float = 0.9
         self.ADAM_BETA2: float = 0.999
@@ -302,6 +327,15 @@ class Config:
             raise ValueError("Must train or load a model.")
         if self.is_loading and not os.path.isdir(self.model_load_dir):
             raise ValueError("Model load dir `{}` does not exist.".format(self.model_load_dir))
+        self.verify_choices()
+
+    def verify_choices(self):
+        for name, choices in (('TRANSFORM', self.TRANSFORMS),
+                              ('GATE_ACTIVATION', self.GATE_ACTIVATIONS),
+                              ('TARGET_FORMAT', self.TARGET_FORMATS)):
+            if getattr(self, name) not in choices:
+                raise ValueError('%s must be one of %s, not %r'
+                                 % (name, ', '.join(choices), getattr(self, name)))
 
     def __iter__(self):
         for attr_name in dir(self):

@@ -5,6 +5,7 @@ is the reference graph (tensorflow_model.py:197-265):
 
     ctx    = dropout(concat(tok[src], path[p], tok[tgt]))        # K1-K3
     comb   = tanh(ctx @ TRANSFORM)                               # K4
+             (or act(ctx @ GATE) * (ctx @ UP): config.TRANSFORM = 'gated')
     code   = Σ_c softmax_c(comb·ATTENTION + log mask) · comb     # K5-K7
     logits = code @ TARGETS^T                                    # K8
     loss   = mean CE(logits, target)                             # K9
@@ -35,6 +36,7 @@ class ForwardState(NamedTuple):
     alpha: torch.Tensor      # (B, C) fp32
     seed: int
     seed_t: Optional[torch.Tensor] = None
+    gu: Optional[torch.Tensor] = None   # kept by the gated transform
 
 
 class NullReducer:
@@ -71,7 +73,9 @@ class Code2VecNetwork:
     def __init__(self, config: Config, token_vocab_size: int,
                  path_vocab_size: int, target_vocab_size: int,
                  device: Optional[str] = None):
+        config.verify_choices()
         self.config = config
+        self.gated = config.TRANSFORM == 'gated'
         self.device = torch.device(device or config.resolve_device())
         self.compute_dtype = (torch.bfloat16 if config.COMPUTE_DTYPE == 'bf16'
                               else torch.float32)
@@ -90,7 +94,9 @@ class Code2VecNetwork:
         self.tok_table = uniform((token_vocab_size, d), math.sqrt(3.0 / d))
         self.path_table = uniform((path_vocab_size, d), math.sqrt(3.0 / d))
         self.target_table = uniform((target_vocab_size, D), math.sqrt(3.0 / D))
-        self.w = uniform((D, D), math.sqrt(6.0 / (D + D)))       # (in, out)
+        # (in, out), or (gate/up, in, out)
+        self.w = uniform((2, D, D) if self.gated else (D, D),
+                         math.sqrt(6.0 / (D + D)))
         self.a = uniform((D,), math.sqrt(6.0 / (D + 1)))
 
         # Adam state (fp32), lazy for the embedding tables.
@@ -122,6 +128,13 @@ class Code2VecNetwork:
             # second side stream: the sparse-grad hash build depends only on
             # the input ids, so it runs under the FORWARD pass
             self._hash_stream = torch.cuda.Stream()
+        # MXFP4 codes of the target table, kept beside it like the shadows and
+        # made again when they are next needed after the table has changed
+        self._target_codes = None
+        self._codes_ready = None
+        if config.TARGET_FORMAT != 'full':
+            self._target_codes = F.mxfp4_quantize(self.target_table)
+            self._targets_changed = True
 
     # ---- parameters ----
 
@@ -142,15 +155,23 @@ class Code2VecNetwork:
         computing with stale capture-time weights (found the hard way — the
         graph-vs-eager test caught a 2e-3 parameter drift)."""
         cd = self.compute_dtype
+        if self.gated:
+            # (2,out,in) and (in, gate's out then up's)
+            w_oi, w_io = self.w.transpose(1, 2), self.w.transpose(0, 1)
+        else:
+            w_oi, w_io = self.w.t(), self.w
         if getattr(self, 'w_oi', None) is None:
-            self.w_oi = self.w.t().contiguous().to(cd)  # (out,in): fwd B^T
-            self.w_io = self.w.contiguous().to(cd)      # (in,out): bwd B^T
+            self.w_oi = w_oi.contiguous().to(cd)        # (out,in): fwd B^T
+            self.w_io = w_io.contiguous().to(cd)        # (in,out): bwd B^T
+            if self.gated:
+                self.w_io = self.w_io.flatten(1)
             self.a_c = self.a.to(torch.float32)
         else:
-            self.w_oi.copy_(self.w.t())
-            self.w_io.copy_(self.w)
+            self.w_oi.copy_(w_oi)
+            self.w_io.view(w_io.shape).copy_(w_io)
             self.a_c.copy_(self.a)
         if not only_w:
+            self._targets_changed = True
             if getattr(self, 'target_shadow', None) is None:
                 self.target_shadow = self.target_table.to(cd)
             else:
@@ -162,6 +183,7 @@ class Code2VecNetwork:
         # dropout stream position: resuming mid-training replays the exact
         # per-step seeds the uninterrupted run would have used
         sd['dropout_step'] = torch.tensor(self._step_ctr)
+        sd.update(self._transform_state())
         for n in self.param_names():
             sd['adam_m.' + n] = self._adam_m[n].cpu()
             sd['adam_v.' + n] = self._adam_v[n].cpu()
@@ -170,9 +192,31 @@ class Code2VecNetwork:
     def weights_state_dict(self) -> Dict[str, torch.Tensor]:
         """Release form: weights only, optimizer state stripped
         (reference release flow, tensorflow_model.py:129-136)."""
-        return {n: self.get_param(n).cpu() for n in self.param_names()}
+        return {**{n: self.get_param(n).cpu() for n in self.param_names()},
+                **self._transform_state()}
+
+    def _transform_state(self) -> Dict[str, torch.Tensor]:
+        # the weights of a gated transform mean nothing without its activation
+        if not self.gated:
+            return {}
+        return {'gate_activation': torch.tensor(
+            F.GATE_ACTIVATIONS.index(self.config.GATE_ACTIVATION))}
+
+    def _check_state(self, sd: Dict[str, torch.Tensor]):
+        for n in self.param_names():
+            want = tuple(self.get_param(n).shape)
+            if tuple(sd[n].shape) != want:
+                raise ValueError(
+                    'the checkpoint holds %s with shape %s, this model (%s transform) '
+                    'has %s' % (n, tuple(sd[n].shape), self.config.TRANSFORM, want))
+        if 'gate_activation' in sd:
+            act = F.GATE_ACTIVATIONS[int(sd['gate_activation'])]
+            if act != self.config.GATE_ACTIVATION:
+                raise ValueError('the checkpoint was trained with %s gates, this model '
+                                 'has %s' % (act, self.config.GATE_ACTIVATION))
 
     def load_state_dict(self, sd: Dict[str, torch.Tensor]):
+        self._check_state(sd)
         for n in self.param_names():
             self.get_param(n).copy_(sd[n].to(self.device))
         if 'dropout_step' in sd:
@@ -218,14 +262,47 @@ class Code2VecNetwork:
                                   out_dtype=self.compute_dtype, seed_t=seed_t)
         if _post_ctx_hook is not None:
             _post_ctx_hook()
-        comb = F.transform_tanh_fwd(ctx, self.w_oi)                  # (B*C, D)
+        comb, gu = self.transform(ctx, save=training)                # (B*C, D)
         code, alpha = F.attention_fwd(comb.reshape(B, C, D), self.a_c, valid_mask)
         return ForwardState(ctx=ctx, comb=comb, code=code, alpha=alpha,
-                            seed=seed, seed_t=seed_t)
+                            seed=seed, seed_t=seed_t, gu=gu)
+
+    def transform(self, ctx: torch.Tensor, save: bool = False):
+        """ctx (N,D) → (comb (N,D), what the gated transform's backward needs
+        if `save`, else None)."""
+        if self.gated:
+            return F.transform_gated_fwd(ctx, self.w_oi,
+                                         self.config.GATE_ACTIVATION, save)
+        return F.transform_tanh_fwd(ctx, self.w_oi), None
+
+    def target_codes(self) -> F.Mxfp4:
+        """The target table in MXFP4 (config.TARGET_FORMAT 'w4' or 'w4a4'), in
+        buffers that keep their place, so that captured graphs may read them."""
+        capturing = (self.device.type == 'cuda'
+                     and torch.cuda.is_current_stream_capturing())
+        if self._targets_changed:
+            q = F.mxfp4_quantize(self.target_table)
+            self._target_codes.codes.copy_(q.codes)
+            self._target_codes.scales.copy_(q.scales)
+            if not capturing:
+                # (a capture has written nothing yet)
+                if self.device.type == 'cuda':
+                    self._codes_ready = torch.cuda.Event()
+                    self._codes_ready.record()
+                self._targets_changed = False
+        elif self._codes_ready is not None and not capturing:
+            # they may have been made on another stream
+            torch.cuda.current_stream().wait_event(self._codes_ready)
+        return self._target_codes
 
     def logits(self, code: torch.Tensor) -> torch.Tensor:
         """code (B,D) fp32 → (B, V_tgt) compute dtype:
-        256-tile MFMA kernel on big shapes, hipBLASLt otherwise."""
+        256-tile MFMA kernel on big shapes, hipBLASLt otherwise; with
+        config.TARGET_FORMAT 'w4' or 'w4a4' from the table's MXFP4 codes."""
+        if self.config.TARGET_FORMAT != 'full':
+            x = (F.mxfp4_quantize(code) if self.config.TARGET_FORMAT == 'w4a4'
+                 else code.to(self.compute_dtype))
+            return F.mxfp4_matmul(x, self.target_codes(), self.compute_dtype)
         return F.logits_gemm(code.to(self.compute_dtype), self.target_shadow)
 
     # ---- full training step ----
@@ -235,6 +312,7 @@ class Code2VecNetwork:
         """One full optimizer step. Returns the (device-resident, unsynced)
         scalar mean loss so callers control when to pay the H2D sync."""
         reducer = reducer or NullReducer()
+        self._targets_changed = True
         cfg = self.config
         B, C = src_ids.shape
         D = cfg.CODE_VECTOR_SIZE
@@ -406,15 +484,26 @@ class Code2VecNetwork:
                     d_target = F.logits_bwd_target(d_logits, code_c)
                 reducer.allreduce_dense('target_table', d_target)
 
-        # attention backward emits dL/dz directly (tanh' fused into its
-        # d_comb write); the dX GEMM applies the dropout mask in its epilogue
-        # — no separate tanh_bwd or dropout_bwd passes
-        d_z3, d_a = F.attention_bwd(st.comb.reshape(B, C, D), self.a_c,
-                                    st.alpha, d_code, fuse_tanh_bwd=True)
-        d_z = d_z3.reshape(B * C, D)
-        d_ctx, d_w = F.linear_bwd_dropout(d_z, self.w_io, st.ctx,
-                                          cfg.DROPOUT_KEEP_RATE, st.seed,
-                                          seed_t=st.seed_t, training=True)
+        if self.gated:
+            # dL/dcomb; the activation's derivative and both projections are
+            # undone by the transform's backward, the dropout mask on the way
+            d_comb, d_a = F.attention_bwd(st.comb.reshape(B, C, D), self.a_c,
+                                          st.alpha, d_code)
+            d_ctx, d_w = F.transform_gated_bwd(
+                st.ctx, self.w_io, st.gu, d_comb.reshape(B * C, D),
+                cfg.GATE_ACTIVATION, cfg.DROPOUT_KEEP_RATE, st.seed,
+                seed_t=st.seed_t)
+            d_w = d_w.float()   # ranks and Adam add in fp32
+        else:
+            # attention backward emits dL/dz directly (tanh' fused into its
+            # d_comb write); the dX GEMM applies the dropout mask in its epilogue
+            # — no separate tanh_bwd or dropout_bwd passes
+            d_z3, d_a = F.attention_bwd(st.comb.reshape(B, C, D), self.a_c,
+                                        st.alpha, d_code, fuse_tanh_bwd=True)
+            d_z = d_z3.reshape(B * C, D)
+            d_ctx, d_w = F.linear_bwd_dropout(d_z, self.w_io, st.ctx,
+                                              cfg.DROPOUT_KEEP_RATE, st.seed,
+                                              seed_t=st.seed_t, training=True)
         reducer.allreduce_dense('w', d_w)
         reducer.allreduce_dense('a', d_a)
 
@@ -646,5 +735,6 @@ class GraphTrainStep:
         self.mask.copy_(mask)
         self.labels.copy_(labels)
         self.graph.replay()
+        self.net._targets_changed = True
         self.net.adam_step_host_sync(+1)
         return self.loss

@@ -114,8 +114,11 @@ class Code2VecModel(Code2VecModelBase):
         slots, or a weights-only `.release`) into the engine."""
         import math
         from ..utils.tf_bundle import TFCheckpointReader
-        reader = TFCheckpointReader(prefix)
         net = self.network
+        if net.gated:
+            raise ValueError('%s is a TF checkpoint: its TRANSFORM is one projection, '
+                             'this model has a gated transform' % prefix)
+        reader = TFCheckpointReader(prefix)
         for tf_name, param_name in self.TF_NAME_MAP.items():
             param = net.get_param(param_name)
             arr = reader.get_tensor(tf_name)
@@ -151,6 +154,10 @@ class Code2VecModel(Code2VecModelBase):
             # weights only, optimizer state stripped (reference release flow)
             torch.save({'model': self.network.weights_state_dict(),
                         'epoch': self._epochs_trained}, path + '.release')
+            if self.network.gated:
+                # a TF graph of the reference has no variable for a gate
+                self.log('Released model saved to: %s' % (path + '.release'))
+                return
             # also emit the TF Saver V2 form so the ORIGINAL reference code
             # (tf.compat.v1.train.Saver.restore) can load models trained
             # here — the inverse of the released-model import path

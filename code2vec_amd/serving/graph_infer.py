@@ -47,9 +47,12 @@ class GraphCapturedPredictor:
         ctx = F.gather_concat_fwd(net.tok_table, net.path_table, self.src,
                                   self.pth, self.tgt, 1.0, 0, False,
                                   out_dtype=net.compute_dtype)
-        comb = F.transform_tanh_fwd(ctx, net.w_oi)
+        comb, _ = net.transform(ctx)
         code, alpha = F.attention_fwd(comb.reshape(B, C, D), net.a_c, self.mask)
-        logits = code.to(net.compute_dtype) @ net.target_shadow.t()
+        if net.config.TARGET_FORMAT == 'full':
+            logits = code.to(net.compute_dtype) @ net.target_shadow.t()
+        else:
+            logits = net.logits(code)
         scores, indices = F.topk(logits, k=self.k)
         return indices, scores, code
 
@@ -67,6 +70,8 @@ class GraphCapturedPredictor:
         if n < self.B:
             self.mask[n:, :].zero_()
             self.mask[n:, 0] = 1.0  # keep padded rows numerically benign
+        if self.net.config.TARGET_FORMAT != 'full':
+            self.net.target_codes()   # the replay reads them as they are
         self.graph.replay()
         idx, scores, code = self.out
         return idx[:n], scores[:n], code[:n]

@@ -22,10 +22,14 @@ def main():
     ap.add_argument('--steps', type=int, default=30)
     ap.add_argument('--warmup', type=int, default=10)
     ap.add_argument('--topk', type=int, default=10)
+    ap.add_argument('--transform', choices=Config.TRANSFORMS, default='tanh')
+    ap.add_argument('--target-format', choices=Config.TARGET_FORMATS, default='full')
     args = ap.parse_args()
 
     assert torch.cuda.is_available()
     cfg = Config(set_defaults=True)
+    cfg.TRANSFORM = args.transform
+    cfg.TARGET_FORMAT = args.target_format
     net = Code2VecNetwork(cfg,
                           token_vocab_size=cfg.MAX_TOKEN_VOCAB_SIZE + 1,
                           path_vocab_size=cfg.MAX_PATH_VOCAB_SIZE + 1,
@@ -70,6 +74,8 @@ def main():
         'eager_ex_per_sec': round(B / eager, 1),
         'graph_ex_per_sec': round(B / graphed, 1),
         'topk': args.topk,
+        'transform': args.transform,
+        'target_format': args.target_format,
         'dtype': 'bf16',
         'data': 'synthetic',
     }))
