@@ -36,7 +36,7 @@ class ForwardState(NamedTuple):
     alpha: torch.Tensor      # (B, C) fp32
     seed: int
     seed_t: Optional[torch.Tensor] = None
-    gu: Optional[torch.Tensor] = None   # kept by the gated transform
+    kept: Optional[torch.Tensor] = None   # by the gated transform
 
 
 class NullReducer:
@@ -262,10 +262,10 @@ class Code2VecNetwork:
                                   out_dtype=self.compute_dtype, seed_t=seed_t)
         if _post_ctx_hook is not None:
             _post_ctx_hook()
-        comb, gu = self.transform(ctx, save=training)                # (B*C, D)
+        comb, kept = self.transform(ctx, save=training)                # (B*C, D)
         code, alpha = F.attention_fwd(comb.reshape(B, C, D), self.a_c, valid_mask)
         return ForwardState(ctx=ctx, comb=comb, code=code, alpha=alpha,
-                            seed=seed, seed_t=seed_t, gu=gu)
+                            seed=seed, seed_t=seed_t, kept=kept)
 
     def transform(self, ctx: torch.Tensor, save: bool = False):
         """ctx (N,D) → (comb (N,D), what the gated transform's backward needs
@@ -490,7 +490,7 @@ class Code2VecNetwork:
             d_comb, d_a = F.attention_bwd(st.comb.reshape(B, C, D), self.a_c,
                                           st.alpha, d_code)
             d_ctx, d_w = F.transform_gated_bwd(
-                st.ctx, self.w_io, st.gu, d_comb.reshape(B * C, D),
+                st.ctx, self.w_io, st.kept, d_comb.reshape(B * C, D),
                 cfg.GATE_ACTIVATION, cfg.DROPOUT_KEEP_RATE, st.seed,
                 seed_t=st.seed_t)
             d_w = d_w.float()   # ranks and Adam add in fp32

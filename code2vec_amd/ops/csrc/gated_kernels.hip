@@ -4,11 +4,14 @@
 //   du = dy * act(g),  dg = dy * u * act'(g)
 //   dx = dg Wg + du Wu,  dW = x^T [dg | du]
 //
-// bf16 operands, fp32 accumulation and fp32 activations. What is rounded to
-// bf16 on the way: g and u as they are kept for the backward, and dg and du
-// as operands of the two products that consume them; each such value enters
-// sums of 2H or N terms, so that a rounding of 2^-9 of a term stays one of
-// about 2^-9 of the result, which is itself rounded to bf16.
+// The backward forms g and u again from x: to write and read them costs as
+// much, or loses precision. (204800 rows, K = H = 384, forward and backward: in
+// fp32 835 us, again 700; 14351 rows, 1440: 565 and 579; in bf16 670 and 476,
+// but with gradients off by 0.0030 where once rounded ones are by 0.0017 and
+// these by 0.0024.) bf16 operands, fp32 accumulation and activations. What is rounded to bf16 on the way are dg
+// and du, as operands of the two products that consume them; each such value
+// enters sums of 2H or N terms, so that a rounding of 2^-9 of a term stays one
+// of about 2^-9 of the result, which is itself rounded to bf16.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -42,7 +45,7 @@ DEVI void act_both(float g, float& a, float& da) {
   if constexpr (ACT == SILU) {
     const float s = sigmoid(g);
     a = g * s;
-    da = s * (1.f + g * (1.f - s));
+    da = s + a * (1.f - s);
   } else if constexpr (ACT == GELU) {
     // erfc and not 1 + erf: far left the sum would leave no digits
     const float cdf = 0.5f * erfcf(g * -0.70710678f);
@@ -95,11 +98,11 @@ DEVI u16x8 pack8(const float* v) {
 // product.
 // ---------------------------------------------------------------------------
 
-// Tiles go from memory into a ring of LDS buffers, one or two steps ahead of
-// the matrix instructions. A step begins when its own tile has arrived, which
-// is when no more than N of the loads and stores that this wave issued after
-// it are outstanding, and when every wave has read the tile that the step's
-// new loads overwrite.
+// Tiles go from memory into a ring of LDS buffers ahead of the matrix
+// instructions. A step begins when its own tile has arrived, which is when no
+// more than N of the loads and stores that this wave issued after it are
+// outstanding, and when every wave has read the tile that the step's new loads
+// overwrite.
 template <int N>
 DEVI void wait_queue() {
   static_assert(N < 64, "vmcnt has 6 bits");
@@ -113,14 +116,15 @@ DEVI void block_barrier() {
   asm volatile("" ::: "memory");
 }
 
-enum Epilogue : int { GATED = 0, PLAIN = 1 };
+// GATED: y; DGATED: dg and du
+enum Epilogue : int { GATED = 0, PLAIN = 1, DGATED = 2 };
 
 struct BtArgs {
   const ushort* x;    // (N, K), rows ldx apart
-  const ushort* w;    // GATED: (2, H, K); PLAIN: (H, K)
-  ushort* y;          // (N, H)
-  ushort* gu;         // GATED: (N, 2, Hp) or null
-  long ldx;
+  const ushort* w;    // (2, H, K); PLAIN: (H, K)
+  ushort* y;          // (N, H); DGATED: dgu (N, 2, Hp)
+  const ushort* dy;   // DGATED: (N, Hp), rows lddy apart, zeros behind H
+  long ldx, lddy;
   int N, H, Hp, K;
   float keep_prob;    // PLAIN with dropout: below one
   u64 seed;
@@ -152,26 +156,60 @@ DEVI void put(ushort* base, const float* v, int h, int H) {
   }
 }
 
+// A lane's columns from h of one row; `to` is where they go.
 template <int ACT, int GT>
-DEVI void put_gated(const BtArgs& p, long n, int h, const f32x4* g, const f32x4* u) {
-  float gv[4 * GT], uv[4 * GT], yv[4 * GT];
+DEVI void put_gated(const BtArgs& p, ushort* to, int h, const f32x4* g, const f32x4* u) {
+  float yv[4 * GT];
 #pragma unroll
   for (int j = 0; j < 4 * GT; ++j) {
-    gv[j] = g[j / 4][j & 3];
-    uv[j] = u[j / 4][j & 3];
     float a, da;
-    act_both<ACT>(gv[j], a, da);
-    yv[j] = a * uv[j];
+    act_both<ACT>(g[j / 4][j & 3], a, da);
+    yv[j] = a * u[j / 4][j & 3];
   }
-  put<GT>(p.y + n * p.H + h, yv, h, p.H);
-  if (p.gu) {
-    put<GT>(p.gu + n * 2 * p.Hp + h, gv, h, p.H);
-    put<GT>(p.gu + n * 2 * p.Hp + p.Hp + h, uv, h, p.H);
+  put<GT>(to, yv, h, p.H);
+}
+
+// the same columns of dy, two a register
+template <int GT>
+struct DyPart {
+  u32 v[2 * GT];
+};
+
+template <int GT>
+DEVI DyPart<GT> read_dy(const BtArgs& p, const ushort* from, int h) {
+  constexpr int W = GT == 1 ? 4 : 8;
+  DyPart<GT> d = {};
+#pragma unroll
+  for (int c = 0; c < 4 * GT; c += W)
+    if (h + c < p.Hp)
+      __builtin_memcpy(d.v + c / 2, __builtin_assume_aligned(from + c, 2 * W), 2 * W);
+  return d;
+}
+
+// what is behind H comes out as zeros, up to Hp
+template <int ACT, int GT>
+DEVI void put_dgated(const BtArgs& p, ushort* to, int h, const f32x4* g, const f32x4* u,
+                     const DyPart<GT>& d) {
+  float dg[4 * GT], du[4 * GT];
+#pragma unroll
+  for (int j = 0; j < 4 * GT; ++j) {
+    float a, da;
+    act_both<ACT>(g[j / 4][j & 3], a, da);
+    const float dy = __builtin_bit_cast(
+        float, j & 1 ? d.v[j / 2] & 0xFFFF0000u : d.v[j / 2] << 16);
+    dg[j] = dy * u[j / 4][j & 3] * da;
+    du[j] = dy * a;
   }
+  if (p.Hp != p.H)
+#pragma unroll
+    for (int j = 0; j < 4 * GT; ++j)
+      if (h + j >= p.H) dg[j] = du[j] = 0.f;
+  put<GT>(to, dg, h, p.Hp);
+  put<GT>(to + p.Hp, du, h, p.Hp);
 }
 
 template <int GT>
-DEVI void put_plain(const BtArgs& p, long n, int h, const f32x4* a) {
+DEVI void put_plain(const BtArgs& p, ushort* to, long n, int h, const f32x4* a) {
   float v[4 * GT];
 #pragma unroll
   for (int j = 0; j < 4 * GT; ++j) v[j] = a[j / 4][j & 3];
@@ -183,7 +221,7 @@ DEVI void put_plain(const BtArgs& p, long n, int h, const f32x4* a) {
       v[j] = hash_uniform(seed, (u64)n * p.H + h + j) < p.keep_prob ? v[j] * inv_keep
                                                                    : 0.f;
   }
-  put<GT>(p.y + n * p.H + h, v, h, p.H);
+  put<GT>(to, v, h, p.H);
 }
 
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK,
@@ -194,11 +232,19 @@ __global__ void k_rows_gemm(BtArgs p) {
   constexpr int BM = WR * XT * 16;         // rows of x a block
   constexpr int BG = WC * GT * 16;         // columns of one group
   constexpr int BN = 2 * BG;               // rows of w a block
-  constexpr int HT = EPI == GATED ? BG : BN;   // output columns a block
+  constexpr int HT = EPI == PLAIN ? BN : BG;   // output columns a block
   constexpr int CH = BK / 8;               // 16-byte chunks a row
   constexpr int IT = (BM + BN) * CH / T;
+  // Operands of one half of a step are read while the other half is multiplied,
+  // those of a step's first half behind a barrier in the middle of the step
+  // before. For the largest tile there are not registers enough; its steps begin
+  // with their barrier. (The gated product of 50000 rows, K = H = 640, tiles of
+  // 128 by 64: 89 us, with the barriers between the steps 98; 204800 rows of 384:
+  // 176 and 180. The largest: 240 with spills, and 163.)
+  constexpr bool PIPE = GT < 4;
+  static_assert(BK == 64 && (PIPE || STAGES == 2), "two halves a step");
   // where a row's 16-byte chunks lie: 8 rows read at once cover all banks
-  auto place = [](int row) { return BK == 64 ? row & 7 : (row >> 1) & 3; };
+  auto place = [](int row) { return row & 7; };
   constexpr int ITX = BM * CH / T;         // of them from x
   static_assert(BM * CH % T == 0 && BN * CH % T == 0, "staging");
   extern __shared__ ushort lds[];          // STAGES x (BM + BN) x BK
@@ -246,10 +292,10 @@ __global__ void k_rows_gemm(BtArgs p) {
         const int grp = (j >> 4) / GT % 2, cw = (j >> 4) / (2 * GT);
         const int in_group = (i >> 2) * (4 * GT) + mi * 4 + (i & 3);
         long wrow;
-        if constexpr (EPI == GATED)
-          wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
-        else
+        if constexpr (EPI == PLAIN)
           wrow = min(h0 + (cw * 2 + grp) * GT * 16 + in_group, p.H - 1);
+        else
+          wrow = (long)grp * p.H + min(h0 + cw * GT * 16 + in_group, p.H - 1);
         off[it] = (u32)(wrow * p.K * 2) + col;
       }
     }
@@ -274,78 +320,162 @@ __global__ void k_rows_gemm(BtArgs p) {
   };
 
   // stores of a wave in a tile's end, where all of it is there
-  constexpr int PUT = XT * (GT >= 2 ? GT / 2 : 1);
+  constexpr int PUT = XT * (GT >= 2 ? GT / 2 : 1) * (EPI == GATED ? 1 : 2);
   const int steps = (p.K + BK - 1) / BK;
-  bool whole = false;                      // the tile before was
+
+  // What is asked for runs ahead of what is multiplied, from one tile into the
+  // next: of `ltile` the step `lstep` is next, and `ahead` steps that were
+  // asked for have not been waited for.
+  int ltile = tile, lstep = 0, lbuf = 0, ahead = 0;
+  auto ask = [&](bool always) {
+    if (lstep == steps && ltile < tile1) {
+      ltile += each;
+      lstep = 0;
+      if (ltile < tile1) begin(ltile);
+    }
+    const bool any = ltile < tile1;
+    if (!any && !always) return;
+    stage((any ? lstep : 0) * BK, lbuf);
+    lbuf = lbuf == STAGES - 1 ? 0 : lbuf + 1;
+    lstep += any;
+    ahead += any;
+  };
+  // The next step is there: behind it in the queue are the steps that were asked
+  // for after it and perhaps the stores of the tile before. Every wave has read
+  // the step before it, whose buffer is the next to fill.
+  auto arrive = [&](bool stores) {
+    if (STAGES == 3 && ahead == 3) {
+      wait_queue<2 * IT>();
+    } else if (ahead >= 2) {
+      if (stores) wait_queue<IT + PUT>();
+      else wait_queue<IT>();
+    } else {
+      if (stores) wait_queue<PUT>();
+      else wait_queue<0>();
+    }
+    block_barrier();
+    --ahead;
+  };
   int buf = 0;
+  struct Half { bf16x8 x[XT], w[2 * GT]; };
+  auto read = [&](Half& f, int kk) {
+    const ushort* xs = lds + buf * (BM + BN) * BK + wr * XT * 16 * BK;
+    const ushort* ws = lds + buf * (BM + BN) * BK + (BM + wc * 2 * GT * 16) * BK;
+    const int off = l16 * BK + (((kk * 4 + q) ^ place(l16)) * 8);
+#pragma unroll
+    for (int i = 0; i < XT; ++i)
+      f.x[i] = *reinterpret_cast<const bf16x8*>(xs + i * 16 * BK + off);
+#pragma unroll
+    for (int j = 0; j < 2 * GT; ++j)
+      f.w[j] = *reinterpret_cast<const bf16x8*>(ws + j * 16 * BK + off);
+  };
+  bool whole = false;                      // the tile before was
   begin(tile);
-  stage(0, 0);
-  if (STAGES == 3 && steps > 1) stage(BK, 1);
-  for (;;) {
+#pragma unroll 1
+  for (int s = 0; s < STAGES; ++s) ask(false);
+  Half f, g;
+  if (PIPE) {
+    arrive(false);
+    read(f, 0);
+  }
+  for (; tile < tile1; tile += each) {
     f32x4 acc[XT][2 * GT];
 #pragma unroll
     for (int i = 0; i < XT; ++i)
 #pragma unroll
       for (int j = 0; j < 2 * GT; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
-    long row = row0;
-    int h = h0;
-    const bool more = STAGES == 2 && tile + each < tile1;
-    for (int s = 0; s < steps; ++s) {
-      if (STAGES == 3 ? s + 1 < steps : false) {
-        wait_queue<IT>();
-      } else if (STAGES == 2 && s == 0 && whole) {
-        // the stores of the tile before are behind this tile's loads
-        if (EPI == PLAIN) wait_queue<2 * PUT>();
-        else if (p.gu) wait_queue<3 * PUT>();
-        else wait_queue<PUT>();
-      } else {
-        wait_queue<0>();
-      }
-      block_barrier();
-      const int into = STAGES == 2 ? buf ^ 1 : buf == 0 ? 2 : buf - 1;
-      if (s + STAGES - 1 < steps) {
-        stage((s + STAGES - 1) * BK, into);
-      } else if (more) {
-        begin(tile + each);
-        stage(0, into);
-      }
-      const ushort* xs = lds + buf * (BM + BN) * BK + wr * XT * 16 * BK;
-      const ushort* ws = lds + buf * (BM + BN) * BK +
-                         (BM + wc * 2 * GT * 16) * BK;
-      buf = buf == STAGES - 1 ? 0 : buf + 1;
+    const long row = row0;
+    const int h = h0;
+    auto multiply = [&](const Half& f) {
 #pragma unroll
-      for (int kk = 0; kk < BK / 32; ++kk) {
-        const int off = l16 * BK + (((kk * 4 + q) ^ place(l16)) * 8);
-        bf16x8 xf[XT], wf[2 * GT];
-#pragma unroll
-        for (int i = 0; i < XT; ++i)
-          xf[i] = *reinterpret_cast<const bf16x8*>(xs + i * 16 * BK + off);
+      for (int i = 0; i < XT; ++i)
 #pragma unroll
         for (int j = 0; j < 2 * GT; ++j)
-          wf[j] = *reinterpret_cast<const bf16x8*>(ws + j * 16 * BK + off);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[j], f.x[i], acc[i][j],
+                                                              0, 0, 0);
+    };
+    auto flip = [&] { buf = buf == STAGES - 1 ? 0 : buf + 1; };
+    for (int s = 0; s < steps - 1; ++s) {
+      if (PIPE) {
+        read(g, 1);
+        multiply(f);
+        arrive(whole && s < STAGES - 1);
+        flip();
+        ask(false);
+        read(f, 0);
+        multiply(g);
+      } else {
+        arrive(whole && s < STAGES);
+        // (the other buffer holds step 1 when step 0 begins)
+        if (s > 0) ask(false);
+        read(f, 0);
+        read(g, 1);
+        multiply(f);
+        multiply(g);
+        flip();
+      }
+    }
+    // A lane's columns in its rows of the tile, and their places behind the
+    // tile's first row.
+    const int hl = h + (EPI == PLAIN ? 2 : 1) * wc * GT * 16 + q * 4 * GT;
+    const int r = wr * XT * 16 + l16;
+    const int ldy = EPI == DGATED ? 2 * p.Hp : p.H;
+    const u32 at = ((u32)r * ldy + hl) * 2;
+    // The last step. What is asked for behind the stores arrives after them: the
+    // next tile's first steps go ahead, and dy ahead of those. (With dy, a
+    // block's last tile asks for a step in vain: a number of loads that is always
+    // the same is one that can be waited for.)
+    DyPart<GT> dy[EPI == DGATED ? XT : 1];
+    if constexpr (PIPE) {
+      read(g, 1);
+      multiply(f);
+      const bool next = tile + each < tile1;
+      if (next) {
+        arrive(whole && steps - 1 < STAGES - 1);
+        flip();
+      }
+      if constexpr (EPI == DGATED) {
+        const char* dyb = reinterpret_cast<const char*>(p.dy + row * p.lddy);
 #pragma unroll
         for (int i = 0; i < XT; ++i)
-#pragma unroll
-          for (int j = 0; j < 2 * GT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                wf[j], xf[i], acc[i][j], 0, 0, 0);
+          dy[i] = read_dy<GT>(p, reinterpret_cast<const ushort*>(dyb + (u32)(
+              min((long)r + i * 16, p.N - 1 - row) * p.lddy + hl) * 2), hl);
+        asm volatile("" ::: "memory");
       }
+      ask(EPI == DGATED);
+      if (next) read(f, 0);
+      multiply(g);
+    } else {
+      static_assert(EPI != DGATED, "dy is read by the other order");
+      arrive(whole && steps - 1 < STAGES);
+      ask(false);
+      read(f, 0);
+      read(g, 1);
+      multiply(f);
+      multiply(g);
+      flip();
+      asm volatile("" ::: "memory");
+      block_barrier();
+      ask(false);
     }
 #pragma unroll
     for (int i = 0; i < XT; ++i) {
-      const long n = row + wr * XT * 16 + i * 16 + l16;
+      const long n = row + r + i * 16;
       if (n >= p.N) continue;
+      ushort* to = reinterpret_cast<ushort*>(
+          reinterpret_cast<char*>(p.y + (row + i * 16) * ldy) + at);
       if constexpr (EPI == GATED) {
-        put_gated<ACT, GT>(p, n, h + wc * GT * 16 + q * 4 * GT, acc[i], acc[i] + GT);
+        put_gated<ACT, GT>(p, to, hl, acc[i], acc[i] + GT);
+      } else if constexpr (EPI == DGATED) {
+        put_dgated<ACT, GT>(p, to, hl, acc[i], acc[i] + GT, dy[i]);
       } else {
-        put_plain<GT>(p, n, h + wc * 2 * GT * 16 + q * 4 * GT, acc[i]);
-        put_plain<GT>(p, n, h + (wc * 2 + 1) * GT * 16 + q * 4 * GT, acc[i] + GT);
+        put_plain<GT>(p, to, n, hl, acc[i]);
+        put_plain<GT>(p, to + GT * 16, n, hl + GT * 16, acc[i] + GT);
       }
     }
-    if (!more) return;
     whole = row + BM <= p.N && h + HT <= p.H && p.H % (GT == 1 ? 4 : 8) == 0;
-    tile += each;
   }
+  if (EPI == DGATED) wait_queue<0>();
 }
 
 // The same for few rows of x. Bound by reading w, and by how long that takes
@@ -356,7 +486,7 @@ __global__ void k_rows_gemm(BtArgs p) {
 template <int EPI, int ACT, int XT>
 __launch_bounds__(256)
 __global__ void k_rows_skinny(BtArgs p) {
-  constexpr int HT = EPI == GATED ? 16 : 32;
+  constexpr int HT = EPI == PLAIN ? 32 : 16;
   __shared__ f32x4 sums[4][XT][2][64];
   const int nC = (p.H + HT - 1) / HT;
   const int wg = xcd_chunked(blockIdx.x, gridDim.x);
@@ -372,8 +502,8 @@ __global__ void k_rows_skinny(BtArgs p) {
     x[i] = p.x + min(row0 + i * 16 + l16, (long)p.N - 1) * p.ldx;
 #pragma unroll
   for (int g = 0; g < 2; ++g)
-    w[g] = p.w + (EPI == GATED ? (long)g * p.H + min(h0 + l16, p.H - 1)
-                               : (long)min(h0 + g * 16 + l16, p.H - 1)) * p.K;
+    w[g] = p.w + (EPI == PLAIN ? (long)min(h0 + g * 16 + l16, p.H - 1)
+                               : (long)g * p.H + min(h0 + l16, p.H - 1)) * p.K;
   struct Step { bf16x8 x[XT], w[2]; };
   auto load = [&](int s) {
     const int k = s * 32 + q * 8;
@@ -422,56 +552,15 @@ __global__ void k_rows_skinny(BtArgs p) {
   for (int g = 0; g < 2; ++g)
     v[g] = sums[0][wid][g][lane] + sums[1][wid][g][lane] + sums[2][wid][g][lane] +
            sums[3][wid][g][lane];
+  const int h = h0 + q * 4;
+  ushort* to = p.y + n * (EPI == DGATED ? 2 * p.Hp : p.H) + h;
   if constexpr (EPI == GATED) {
-    put_gated<ACT, 1>(p, n, h0 + q * 4, v, v + 1);
+    put_gated<ACT, 1>(p, to, h, v, v + 1);
+  } else if constexpr (EPI == DGATED) {
+    put_dgated<ACT, 1>(p, to, h, v, v + 1, read_dy<1>(p, p.dy + n * p.lddy + h, h));
   } else {
-    put_plain<1>(p, n, h0 + q * 4, v);
-    put_plain<1>(p, n, h0 + 16 + q * 4, v + 1);
-  }
-}
-
-// ---------------------------------------------------------------------------
-// dg and du from what the forward kept. One pass: reads gu and dy, writes
-// dgu; bound by memory. Columns H..Hp of each half are written as zeros, so
-// that the products below run over whole chunks.
-// ---------------------------------------------------------------------------
-
-template <int ACT>
-__launch_bounds__(256)
-__global__ void k_gated_dgu(const ushort* __restrict__ gu,
-                            const ushort* __restrict__ dy, long lddy,
-                            ushort* __restrict__ dgu, long N, int H, int Hp,
-                            int vec) {
-  const int per_row = Hp / 8;
-  const long total = N * per_row;
-  for (long c = (long)blockIdx.x * 256 + threadIdx.x; c < total;
-       c += (long)gridDim.x * 256) {
-    const long n = c / per_row;
-    const int h = (int)(c % per_row) * 8;
-    const ushort* gp = gu + n * 2 * Hp + h;
-    const u16x8 g8 = *reinterpret_cast<const u16x8*>(gp);
-    const u16x8 u8 = *reinterpret_cast<const u16x8*>(gp + Hp);
-    const ushort* dp = dy + n * lddy + h;
-    u16x8 d8 = {};
-    if (vec) {
-      d8 = *reinterpret_cast<const u16x8*>(dp);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (h + j < H) d8[j] = dp[j];
-    }
-    float dg[8], du[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float a, da;
-      act_both<ACT>(bf2f(g8[j]), a, da);
-      const float d = bf2f(d8[j]);
-      dg[j] = h + j < H ? d * bf2f(u8[j]) * da : 0.f;
-      du[j] = h + j < H ? d * a : 0.f;
-    }
-    ushort* op = dgu + n * 2 * Hp + h;
-    *reinterpret_cast<u16x8*>(op) = pack8(dg);
-    *reinterpret_cast<u16x8*>(op + Hp) = pack8(du);
+    put_plain<1>(p, to, n, h, v);
+    put_plain<1>(p, to + 16, n, h + 16, v + 1);
   }
 }
 
@@ -719,21 +808,23 @@ Rows chunked_rows(const torch::Tensor& t, int cols) {
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK, int STAGES>
 void launch_rows(const BtArgs& a, long slots) {
   constexpr int BM = WR * XT * 16, BG = WC * GT * 16;
-  constexpr int HT = EPI == GATED ? BG : 2 * BG;
+  constexpr int HT = EPI == PLAIN ? 2 * BG : BG;
   constexpr size_t bytes = (size_t)STAGES * (BM + 2 * BG) * BK * sizeof(ushort);
   auto* fn = &k_rows_gemm<EPI, ACT, WR, WC, XT, GT, BK, STAGES>;
   static std::atomic<u64> ready{0};
   allow_lds(fn, bytes, ready);
   const long tiles = ((long)a.N + BM - 1) / BM * ((a.H + HT - 1) / HT);
   TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
-  fn<<<(int)std::min(tiles, STAGES == 2 ? slots : tiles), WR * WC * 64, bytes,
+  // (asking ahead goes into the next tile, not into the one after that)
+  const bool stay = (a.K + BK - 1) / BK >= STAGES;
+  fn<<<(int)(stay ? std::min(tiles, slots) : tiles), WR * WC * 64, bytes,
        cur_stream()>>>(a);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
 template <int EPI, int ACT, int XT>
 void launch_skinny(const BtArgs& a) {
-  constexpr int HT = EPI == GATED ? 16 : 32;
+  constexpr int HT = EPI == PLAIN ? 32 : 16;
   const long tiles = ((long)a.N + XT * 16 - 1) / (XT * 16) * ((a.H + HT - 1) / HT);
   TORCH_CHECK(tiles < (1L << 31), "too many tiles for one launch");
   auto* fn = &k_rows_skinny<EPI, ACT, XT>;
@@ -770,8 +861,10 @@ void rows_gemm(const BtArgs& a) {
       launch_us(blocks(128, 64), 512, k64, 0.60, 1.25, 3.0),
       launch_us(blocks(64, 32), 768, k64, 0.30, 0.85, 2.0),
       launch_us(blocks(a.N <= 16 ? 16 : 32, 16), 1024, k32, 0.045, 0.36, 2.6)};
-  switch (std::min_element(us, us + 4) - us) {
-    case 0: return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a, 256);
+  const int first = EPI == GATED ? 0 : 1;
+  switch (std::min_element(us + first, us + 4) - us) {
+    case 0:
+      if constexpr (EPI == GATED) return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a, 256);
     case 1: return launch_rows<EPI, ACT, 2, 2, 4, 2, 64, 2>(a, 512);
     case 2: return launch_rows<EPI, ACT, 2, 2, 2, 1, 64, 3>(a, 768);
     default:
@@ -823,15 +916,6 @@ void launch_dw(const torch::Tensor& d_w, const ushort* dgu, const Rows& x, long 
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
-template <int ACT>
-void launch_dgu(const ushort* gu, const ushort* dy, long lddy, ushort* dgu,
-                long N, int H, int Hp, int vec) {
-  auto* fn = &k_gated_dgu<ACT>;
-  fn<<<grid_of(N * (Hp / 8), 256, 8192), 256, 0, cur_stream()>>>(
-      gu, dy, lddy, dgu, N, H, Hp, vec);
-  C10_HIP_KERNEL_LAUNCH_CHECK();
-}
-
 #define WITH_ACT(act, ...)                                              \
   switch (act) {                                                        \
     case SILU: { constexpr int A = SILU; __VA_ARGS__; break; }          \
@@ -842,45 +926,42 @@ void launch_dgu(const ushort* gu, const ushort* dy, long lddy, ushort* dgu,
     default: TORCH_CHECK(false, "unknown activation ", act);            \
   }
 
-// y (N,H), and gu (N,2,Hp) when it is kept (empty otherwise)
-std::vector<torch::Tensor> transform_gated_fwd(torch::Tensor ctx,
-                                               torch::Tensor w_oi, int64_t act,
-                                               bool save) {
+// y (N,H)
+torch::Tensor transform_gated_fwd(torch::Tensor ctx, torch::Tensor w_oi, int64_t act) {
   check_bf16(ctx, "ctx", 2, ctx);
   check_bf16(w_oi, "w_oi", 3, ctx);
   TORCH_CHECK(w_oi.size(0) == 2 && w_oi.size(2) == ctx.size(1) &&
               w_oi.is_contiguous(), "w_oi must be a contiguous (2, H, K)");
   check_size(ctx.size(0), ctx.size(1), w_oi.size(1));
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
-  const int N = ctx.size(0), K = ctx.size(1), H = w_oi.size(1), Hp = pad8(H);
+  const int N = ctx.size(0), K = ctx.size(1), H = w_oi.size(1);
   auto y = torch::empty({N, H}, ctx.options());
-  auto gu = torch::empty({save ? N : 0, 2, Hp}, ctx.options());
-  if (N == 0 || H == 0) return {y, gu};
+  if (N == 0 || H == 0) return y;
   const Rows x = chunked_rows(ctx, K), w = chunked_rows(w_oi.view({2L * H, K}), K);
-  BtArgs a{x.p, w.p, bf_mut(y), save ? bf_mut(gu) : nullptr, x.ld, N, H, Hp,
-           pad8(K), 1.f, 0, nullptr};
+  BtArgs a{x.p, w.p, bf_mut(y), nullptr, x.ld, 0, N, H, pad8(H), pad8(K), 1.f, 0,
+           nullptr};
   WITH_ACT(act, (rows_gemm<GATED, A>(a)));
-  return {y, gu};
+  return y;
 }
 
 // d_ctx (N,K) and d_w (2,K,H)
 std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
                                                torch::Tensor w_io,
-                                               torch::Tensor gu,
+                                               torch::Tensor w_oi,
                                                torch::Tensor d_y, int64_t act,
                                                double keep_prob, int64_t seed,
                                                c10::optional<torch::Tensor> seed_t) {
   check_bf16(ctx, "ctx", 2, ctx);
   check_bf16(w_io, "w_io", 2, ctx);
-  check_bf16(gu, "gu", 3, ctx);
   check_bf16(d_y, "d_y", 2, ctx);
   const int N = ctx.size(0), K = ctx.size(1), H = d_y.size(1), Hp = pad8(H);
   check_size(ctx.size(0), ctx.size(1), d_y.size(1));
   TORCH_CHECK(d_y.size(0) == N, "d_y must have as many rows as ctx");
   TORCH_CHECK(w_io.size(0) == K && w_io.size(1) == 2L * H && w_io.is_contiguous(),
               "w_io must be a contiguous (K, 2H)");
-  TORCH_CHECK(gu.size(0) == N && gu.size(1) == 2 && gu.size(2) == Hp &&
-              gu.is_contiguous(), "gu must be what the forward kept");
+  check_bf16(w_oi, "w_oi", 3, ctx);
+  TORCH_CHECK(w_oi.size(0) == 2 && w_oi.size(1) == H && w_oi.size(2) == K &&
+              w_oi.is_contiguous(), "w_oi must be a contiguous (2, H, K)");
   TORCH_CHECK(keep_prob > 0.0 && keep_prob <= 1.0, "keep_prob must be in (0, 1]");
   const long* seed_ptr = nullptr;
   if (seed_t) {
@@ -894,15 +975,14 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   if (N == 0 || H == 0 || K == 0)
     return {d_ctx.zero_(), torch::zeros({2, K, H}, ctx.options())};
 
-  auto dgu = torch::empty_like(gu);
+  const Rows x = chunked_rows(ctx, K);
+  auto dgu = torch::empty({N, 2, Hp}, ctx.options());
   {
-    const bool dense = H == 1 || d_y.stride(1) == 1;
-    auto dy = dense ? d_y : d_y.contiguous();
-    const long lddy = N == 1 ? H : dy.stride(0);
-    const int vec = H % 8 == 0 && lddy % 8 == 0 &&
-                    (reinterpret_cast<uintptr_t>(dy.data_ptr()) & 15) == 0;
-    WITH_ACT(act, launch_dgu<A>(bf_ptr(gu), bf_ptr(dy), lddy, bf_mut(dgu), N, H,
-                                Hp, vec));
+    const Rows dy = chunked_rows(d_y, H);
+    const Rows w = chunked_rows(w_oi.view({2L * H, K}), K);
+    BtArgs a{x.p, w.p, bf_mut(dgu), dy.p, x.ld, dy.ld, N, H, Hp, pad8(K), 1.f, 0,
+             nullptr};
+    WITH_ACT(act, (rows_gemm<DGATED, A>(a)));
   }
 
   Rows w;
@@ -911,11 +991,10 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   } else {
     w = chunked_rows(w_io.view({2L * K, H}), H);   // (K, 2, Hp)
   }
-  BtArgs a{bf_ptr(dgu), w.p, bf_mut(d_ctx), nullptr, 2L * Hp, N, K, pad8(K),
-           2 * Hp, (float)keep_prob, (u64)seed, seed_ptr};
+  BtArgs a{bf_ptr(dgu), w.p, bf_mut(d_ctx), nullptr, 2L * Hp, 0, N, K,
+           pad8(K), 2 * Hp, (float)keep_prob, (u64)seed, seed_ptr};
   rows_gemm<PLAIN, SILU>(a);
 
-  const Rows x = chunked_rows(ctx, K);
   auto d_w = torch::empty({2, K, H}, ctx.options());
   const DwPlan large = plan_dw(N, 2L * Hp, K, 256, 128, 512, 0.6, 1.3);
   const DwPlan small = plan_dw(N, 2L * Hp, K, 64, 64, 1024, 0.3, 0.6);

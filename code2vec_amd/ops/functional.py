@@ -76,9 +76,10 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
 
     ctx (N,K); w_oi (2,H,K), gate then up, out-major like the tanh
     transform's shadow; activation one of GATE_ACTIVATIONS. Returns (y (N,H),
-    gu): gu holds what transform_gated_bwd needs if `save`, else None. On the
-    GPU all are bfloat16 (sums and activation in fp32), any N, K and H; rows
-    of ctx may be any stride apart."""
+    kept): kept is what transform_gated_bwd needs if `save`, else None. It is
+    w_oi itself, which must not change in between: to form the projections again
+    takes no longer than to keep them in full. On the GPU all are bfloat16 (sums
+    and activation in fp32), any N, K and H; rows of ctx may be any stride apart."""
     if activation not in GATE_ACTIVATIONS:
         _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
     if (ctx.dim() != 2 or w_oi.dim() != 3 or w_oi.shape[0] != 2
@@ -88,17 +89,18 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
     if ctx.dtype != w_oi.dtype or ctx.device != w_oi.device:
         _refuse('ctx and w_oi must have one type and one device')
     if backend_for(ctx) == 'hip':
-        y, gu = hip_ext(True).transform_gated_fwd(
-            ctx, w_oi, GATE_ACTIVATIONS.index(activation), bool(save))
-        return y, gu if save else None
-    return ref.transform_gated_fwd(ctx, w_oi, activation, save)
+        y = hip_ext(True).transform_gated_fwd(ctx, w_oi,
+                                              GATE_ACTIVATIONS.index(activation))
+    else:
+        y = ref.transform_gated_fwd(ctx, w_oi, activation)
+    return y, w_oi if save else None
 
 
-def transform_gated_bwd(ctx, w_io, gu, d_y, activation: str = 'silu',
+def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
                         keep_prob: float = 1.0, seed: int = 0, seed_t=None
                         ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Backward of the gated transform. ctx as in the forward; w_io (K,2H)
-    the same weights in-major, gate columns then up columns; gu what the
+    the same weights in-major, gate columns then up columns; kept what the
     forward kept; d_y (N,H). Returns (d_ctx (N,K), d_w (2,K,H)), in ctx's
     type. With keep_prob < 1 d_ctx goes through the keep mask of the dropout
     that made ctx (gather_concat_fwd with the same seed) on its way out."""
@@ -108,21 +110,21 @@ def transform_gated_bwd(ctx, w_io, gu, d_y, activation: str = 'silu',
             or w_io.shape != (ctx.shape[1], 2 * d_y.shape[1])):
         _refuse('ctx (N,K), w_io (K,2H) and d_y (N,H) do not fit: %s, %s and %s',
                 tuple(ctx.shape), tuple(w_io.shape), tuple(d_y.shape))
-    if gu is None:
+    if kept is None:
         _refuse('the forward kept nothing: call it with save=True')
-    if gu.shape != (ctx.shape[0], 2, -(-d_y.shape[1] // 8) * 8):
-        _refuse('gu is not what the forward of this ctx kept')
-    for t in (w_io, gu, d_y):
+    if kept.shape != (2, d_y.shape[1], ctx.shape[1]):
+        _refuse('the forward of this ctx kept something else')
+    for t in (w_io, kept, d_y):
         if t.dtype != ctx.dtype or t.device != ctx.device:
-            _refuse('ctx, w_io, gu and d_y must have one type and one device')
+            _refuse('ctx, w_io, kept and d_y must have one type and one device')
     if not 0.0 < keep_prob <= 1.0:
         _refuse('keep_prob must be in (0, 1]')
     if backend_for(ctx) == 'hip':
         d_ctx, d_w = hip_ext(True).transform_gated_bwd(
-            ctx, w_io, gu, d_y, GATE_ACTIVATIONS.index(activation), keep_prob,
+            ctx, w_io, kept, d_y, GATE_ACTIVATIONS.index(activation), keep_prob,
             seed, seed_t)
         return d_ctx, d_w
-    d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, gu, d_y, activation)
+    d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, kept, d_y, activation)
     if keep_prob < 1.0:
         if seed_t is not None:
             seed = int(seed_t.item())

@@ -124,32 +124,27 @@ def _wide(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float64 else t.float()
 
 
-def transform_gated_fwd(ctx: torch.Tensor, w_oi: torch.Tensor, activation: str,
-                        save: bool) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """ctx (N,K), w_oi (2,H,K): y (N,H), and (N,2,Hp) g and u in ctx's type
-    (rows padded to a multiple of eight, as the kernels keep them) if they
-    are to be kept for the backward."""
+def transform_gated_fwd(ctx: torch.Tensor, w_oi: torch.Tensor,
+                        activation: str) -> torch.Tensor:
+    """ctx (N,K), w_oi (2,H,K): y (N,H)."""
     x, w = _wide(ctx), _wide(w_oi)
     g, u = x @ w[0].t(), x @ w[1].t()
-    y = (gate_activation(activation, g)[0] * u).to(ctx.dtype)
-    if not save:
-        return y, None
-    gu = torch.nn.functional.pad(torch.stack((g, u), 1), (0, -w.shape[1] % 8))
-    return y, gu.to(ctx.dtype)
+    return (gate_activation(activation, g)[0] * u).to(ctx.dtype)
 
 
-def transform_gated_bwd(ctx: torch.Tensor, w_io: torch.Tensor, gu: torch.Tensor,
+def transform_gated_bwd(ctx: torch.Tensor, w_io: torch.Tensor, w_oi: torch.Tensor,
                         d_y: torch.Tensor, activation: str
                         ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """w_io (K,2H), gu from the forward: d_ctx (N,K) and d_w (2,K,H), in
-    ctx's type. dg = dy u act'(g); du = dy act(g); d_ctx = [dg|du] w_io^T;
-    d_w = ctx^T [dg|du]."""
+    """w_io (K,2H) and w_oi (2,H,K), the same weights: d_ctx (N,K) and d_w
+    (2,K,H), in ctx's type. dg = dy u act'(g); du = dy act(g); d_ctx =
+    [dg|du] w_io^T; d_w = ctx^T [dg|du]."""
     H = d_y.shape[1]
-    g, u, dy = _wide(gu[:, 0, :H]), _wide(gu[:, 1, :H]), _wide(d_y)
+    x, w, dy = _wide(ctx), _wide(w_oi), _wide(d_y)
+    g, u = x @ w[0].t(), x @ w[1].t()
     a, da = gate_activation(activation, g)
     dgu = torch.cat((dy * u * da, dy * a), 1)                  # (N, 2H)
     d_ctx = dgu @ _wide(w_io).t()
-    d_w = _wide(ctx).t() @ dgu                                 # (K, 2H)
+    d_w = x.t() @ dgu                                          # (K, 2H)
     d_w = d_w.reshape(ctx.shape[1], 2, H).permute(1, 0, 2).contiguous()
     return d_ctx.to(ctx.dtype), d_w.to(ctx.dtype)
 

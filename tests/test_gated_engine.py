@@ -105,12 +105,12 @@ def test_the_tanh_engine_is_what_it_was():
     ctx = torch.cat([a.tok_table[src.long()], a.path_table[pth.long()],
                      a.tok_table[tgt.long()]], dim=-1).reshape(B * C, -1)
     assert torch.allclose(st.comb, torch.tanh(ctx @ a.w), atol=1e-5)
-    assert st.gu is None
+    assert st.kept is None
 
 
 def test_forward_for_answers_keeps_nothing():
     st = make_net().forward(*make_batch()[:4], training=False)
-    assert st.gu is None
+    assert st.kept is None
 
 
 def test_checkpoints(tmp_path):

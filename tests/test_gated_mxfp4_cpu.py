@@ -24,8 +24,8 @@ def test_gated_backward_against_differences(act):
     """Central differences in 64 bits with a step of 1e-5: off by about
     step^2 = 1e-10 times a third derivative, and 1e-16 / step = 1e-11."""
     x, w_oi, w_io, dy = gated_inputs()
-    _, gu = F.transform_gated_fwd(x, w_oi, act, save=True)
-    d_ctx, d_w = F.transform_gated_bwd(x, w_io, gu, dy, act)
+    _, kept = F.transform_gated_fwd(x, w_oi, act, save=True)
+    d_ctx, d_w = F.transform_gated_bwd(x, w_io, kept, dy, act)
 
     def loss(xv, wv):
         return float((F.transform_gated_fwd(xv, wv, act)[0] * dy).sum())
@@ -56,18 +56,18 @@ def test_gated_backward_against_autograd(act):
     xr, wr = x.clone().requires_grad_(True), w_oi.clone().requires_grad_(True)
     y = fn(xr @ wr[0].t()) * (xr @ wr[1].t())
     y.backward(dy)
-    got, gu = F.transform_gated_fwd(x, w_oi, act, save=True)
-    d_ctx, d_w = F.transform_gated_bwd(x, w_io, gu, dy, act)
+    got, kept = F.transform_gated_fwd(x, w_oi, act, save=True)
+    d_ctx, d_w = F.transform_gated_bwd(x, w_io, kept, dy, act)
     for a, b in ((got, y.detach()), (d_ctx, xr.grad), (d_w, wr.grad.transpose(1, 2))):
         assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)
 
 
 def test_gated_dropout_mask_is_the_gathers():
     x, w_oi, w_io, dy = gated_inputs(N=40, K=24, H=16, dtype=torch.float32)
-    _, gu = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
-    plain, _ = F.transform_gated_bwd(x, w_io, gu, dy, 'silu')
-    got, _ = F.transform_gated_bwd(x, w_io, gu, dy, 'silu', keep_prob=0.75, seed=77)
-    again, _ = F.transform_gated_bwd(x, w_io, gu, dy, 'silu', keep_prob=0.75,
+    _, kept = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
+    plain, _ = F.transform_gated_bwd(x, w_io, kept, dy, 'silu')
+    got, _ = F.transform_gated_bwd(x, w_io, kept, dy, 'silu', keep_prob=0.75, seed=77)
+    again, _ = F.transform_gated_bwd(x, w_io, kept, dy, 'silu', keep_prob=0.75,
                                      seed_t=torch.tensor([77]))
     mask = R.dropout_keep_mask(77, x.numel(), 0.75, 'cpu').reshape(x.shape)
     assert torch.equal(got, again)
@@ -77,8 +77,8 @@ def test_gated_dropout_mask_is_the_gathers():
 
 def test_gated_refusals():
     x, w_oi, w_io, dy = gated_inputs()
-    y, gu = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
-    assert y.shape == (5, 11) and gu.shape == (5, 2, 16)
+    y, kept = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
+    assert y.shape == (5, 11) and torch.equal(kept, w_oi)
     assert F.transform_gated_fwd(x, w_oi)[1] is None
     for bad in (lambda: F.transform_gated_fwd(x, w_oi, 'softplus'),
                 lambda: F.transform_gated_fwd(x, w_oi[:1]),
@@ -86,14 +86,14 @@ def test_gated_refusals():
                 lambda: F.transform_gated_fwd(x[0], w_oi),
                 lambda: F.transform_gated_fwd(x.float(), w_oi),
                 lambda: F.transform_gated_bwd(x, w_io, None, dy),
-                lambda: F.transform_gated_bwd(x, w_io, gu[:4], dy),
-                lambda: F.transform_gated_bwd(x, w_io, gu[..., :11], dy),
-                lambda: F.transform_gated_bwd(x, w_io.t(), gu, dy),
-                lambda: F.transform_gated_bwd(x, w_io, gu, dy[:4]),
-                lambda: F.transform_gated_bwd(x, w_io, gu, dy.float()),
-                lambda: F.transform_gated_bwd(x, w_io, gu, dy, 'swish'),
-                lambda: F.transform_gated_bwd(x, w_io, gu, dy, keep_prob=0.0),
-                lambda: F.transform_gated_bwd(x, w_io, gu, dy, keep_prob=1.5)):
+                lambda: F.transform_gated_bwd(x, w_io, kept[:1], dy),
+                lambda: F.transform_gated_bwd(x, w_io, kept[..., :5], dy),
+                lambda: F.transform_gated_bwd(x, w_io.t(), kept, dy),
+                lambda: F.transform_gated_bwd(x, w_io, kept, dy[:4]),
+                lambda: F.transform_gated_bwd(x, w_io, kept, dy.float()),
+                lambda: F.transform_gated_bwd(x, w_io, kept, dy, 'swish'),
+                lambda: F.transform_gated_bwd(x, w_io, kept, dy, keep_prob=0.0),
+                lambda: F.transform_gated_bwd(x, w_io, kept, dy, keep_prob=1.5)):
         with pytest.raises(ValueError):
             bad()
 
