@@ -237,11 +237,12 @@ __global__ void k_rows_gemm(BtArgs p) {
   constexpr int IT = (BM + BN) * CH / T;
   // Operands of one half of a step are read while the other half is multiplied,
   // those of a step's first half behind a barrier in the middle of the step
-  // before. For the largest tile there are not registers enough; its steps begin
-  // with their barrier. (The gated product of 50000 rows, K = H = 640, tiles of
-  // 128 by 64: 89 us, with the barriers between the steps 98; 204800 rows of 384:
-  // 176 and 180. The largest: 240 with spills, and 163.)
-  constexpr bool PIPE = GT < 4;
+  // before. For the largest tile there are not registers enough, and with dy the
+  // compiler finds no good order; their steps begin with their barrier. (Gated,
+  // 50000 rows, K = H = 640, tiles of 128 by 64: 89 us, with the barriers between
+  // the steps 98; the largest tile, 204800 rows of 384: 240 with spills, and 163;
+  // with dy, tiles of 128 by 64: 257, and 241.)
+  constexpr bool PIPE = GT == 1 || (GT == 2 && EPI != DGATED);
   static_assert(BK == 64 && (PIPE || STAGES == 2), "two halves a step");
   // where a row's 16-byte chunks lie: 8 rows read at once cover all banks
   auto place = [](int row) { return row & 7; };
@@ -426,14 +427,7 @@ __global__ void k_rows_gemm(BtArgs p) {
     // block's last tile asks for a step in vain: a number of loads that is always
     // the same is one that can be waited for.)
     DyPart<GT> dy[EPI == DGATED ? XT : 1];
-    if constexpr (PIPE) {
-      read(g, 1);
-      multiply(f);
-      const bool next = tile + each < tile1;
-      if (next) {
-        arrive(whole && steps - 1 < STAGES - 1);
-        flip();
-      }
+    auto ask_dy = [&] {
       if constexpr (EPI == DGATED) {
         const char* dyb = reinterpret_cast<const char*>(p.dy + row * p.lddy);
 #pragma unroll
@@ -442,13 +436,23 @@ __global__ void k_rows_gemm(BtArgs p) {
               min((long)r + i * 16, p.N - 1 - row) * p.lddy + hl) * 2), hl);
         asm volatile("" ::: "memory");
       }
+    };
+    if (PIPE) {
+      read(g, 1);
+      multiply(f);
+      const bool next = tile + each < tile1;
+      if (next) {
+        arrive(whole && steps - 1 < STAGES - 1);
+        flip();
+      }
+      ask_dy();
       ask(EPI == DGATED);
       if (next) read(f, 0);
       multiply(g);
     } else {
-      static_assert(EPI != DGATED, "dy is read by the other order");
       arrive(whole && steps - 1 < STAGES);
-      ask(false);
+      ask_dy();
+      ask(EPI == DGATED);
       read(f, 0);
       read(g, 1);
       multiply(f);
@@ -456,10 +460,15 @@ __global__ void k_rows_gemm(BtArgs p) {
       flip();
       asm volatile("" ::: "memory");
       block_barrier();
-      ask(false);
+      ask(EPI == DGATED);
     }
 #pragma unroll
     for (int i = 0; i < XT; ++i) {
+      // (of the largest tile one row after the other, for want of registers)
+      if (EPI == DGATED && GT == 4) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
       const long n = row + r + i * 16;
       if (n >= p.N) continue;
       ushort* to = reinterpret_cast<ushort*>(
@@ -861,10 +870,10 @@ void rows_gemm(const BtArgs& a) {
       launch_us(blocks(128, 64), 512, k64, 0.60, 1.25, 3.0),
       launch_us(blocks(64, 32), 768, k64, 0.30, 0.85, 2.0),
       launch_us(blocks(a.N <= 16 ? 16 : 32, 16), 1024, k32, 0.045, 0.36, 2.6)};
-  const int first = EPI == GATED ? 0 : 1;
+  const int first = EPI == PLAIN ? 1 : 0;
   switch (std::min_element(us + first, us + 4) - us) {
     case 0:
-      if constexpr (EPI == GATED) return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a, 256);
+      if constexpr (EPI != PLAIN) return launch_rows<EPI, ACT, 4, 2, 4, 4, 64, 2>(a, 256);
     case 1: return launch_rows<EPI, ACT, 2, 2, 4, 2, 64, 2>(a, 512);
     case 2: return launch_rows<EPI, ACT, 2, 2, 2, 1, 64, 3>(a, 768);
     default:
