@@ -14,8 +14,6 @@
 // of about 2^-9 of the result, which is itself rounded to bf16.
 
 #include <torch/extension.h>
-#include <ATen/hip/HIPContext.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 
 #include "c2v_device.h"
 #include "c2v_launch.h"
@@ -224,6 +222,13 @@ DEVI void put_plain(const BtArgs& p, ushort* to, long n, int h, const f32x4* a) 
   put<GT>(to, v, h, p.H);
 }
 
+// 204800 rows, K = H = 384: y 154 us (780 TFLOP/s), dg and du 217 us, dx 162 us;
+// 14351 rows of 1440: 135, 152 and 126 us (880, 780 and 950 TFLOP/s). The
+// matrix units are busy for 4/10 of the time (counted), which is 6/10 of what they
+// sustain without any loads, LDS for as long: a wave reads 12 KB for 32 products of
+// 16 cycles. Rounds of all blocks load, multiply and store in step, so that what
+// moves (314 MB for y, 630 for dg and du, at 5 TB/s) adds to that in part. The
+// epilogue of dg and du takes 18 vector instructions an element, 36 us in all.
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK,
           int STAGES>
 __launch_bounds__(WR * WC * 64, 2)
@@ -491,7 +496,8 @@ __global__ void k_rows_gemm(BtArgs p) {
 // one after the other: a block's four waves share 16 columns (of gate and up;
 // 32 of a plain product) and cut the reduction, step by step in turn; their
 // sums are added in order in LDS. Operands go from memory to registers, two
-// steps ahead.
+// steps ahead. (200 rows, K = H = 384: 4.6 us, where the tiles of 64 by 32 take
+// 4.7 and an empty launch 2.)
 template <int EPI, int ACT, int XT>
 __launch_bounds__(256)
 __global__ void k_rows_skinny(BtArgs p) {
@@ -582,6 +588,10 @@ __global__ void k_rows_skinny(BtArgs p) {
 // neighbouring rows, whose 32-byte units the exclusive-or below spreads over
 // all banks. N is split over blocks; the parts are added in order by
 // k_dw_reduce, so that a result never depends on timing.
+// 204800 rows, K = H = 384: 170 us (710 TFLOP/s, 472 MB read and 66 written),
+// the parts' sum 18 us; 14351 rows of 1440: 158 us (750 TFLOP/s) and 11. Bound as
+// the products above. Reading the next step's operands ahead needs registers that
+// the sums take (272 us with spills; with sums of 192 by 128, 211).
 // ---------------------------------------------------------------------------
 
 constexpr int TN_ROWS = 32;
@@ -851,13 +861,16 @@ double launch_us(double blocks, double slots, double steps, double alone,
 
 // Tiles from 256 rows by 128 columns of gate and up down to 16 by 16: large
 // ones read least, small ones fill the chip. The rates are fitted to both
-// products at 1..204800 rows and widths of 96..1440; what they choose is
-// within a tenth of the best of these at three sizes of four. In us, by tile:
+// products at 1..204800 rows and widths of 96..1440; what they choose is the
+// best or within a tenth of it at six sizes of seven. The gated product, in us:
 //   rows  width   256x128   128x64   64x32   32x16
-//    200    384      14.7      6.9     4.5     4.0
-//   1024    768      24.3     11.3     8.1    19.3
-//   4096   1440      45.2     49.3    84.5   201
-// 204800    384       214      245     359    906
+//    200    384      13.1      6.7     4.7     4.6
+//   1024    768      22.9     11.3     8.7    19.5
+//   4096   1440      47.8     48.5    83.8   182
+//  14351   1440       135      144     257    624
+// 204800    384       154      168     279    906
+// A plain product of the largest tile needs more registers than there are
+// (K = 768 to H = 384, 204800 rows: 207 us, in tiles of 128 by 128 162).
 template <int EPI, int ACT>
 void rows_gemm(const BtArgs& a) {
   constexpr double plain = EPI == PLAIN ? 2 : 1;    // groups of columns a tile
