@@ -14,12 +14,13 @@ from math import ceil
 from typing import Optional
 
 
+TRANSFORMS = ('tanh', 'gated')
+GATE_ACTIVATIONS = ('silu', 'gelu', 'sigmoid', 'tanh', 'relu')
+TARGET_FORMATS = ('full', 'w4', 'w4a4')
+
+
 class Config:
     """All knobs in one object, passed to every layer (reference: config.py:9)."""
-
-    TRANSFORMS = ('tanh', 'gated')
-    GATE_ACTIVATIONS = ('silu', 'gelu', 'sigmoid', 'relu', 'tanh')
-    TARGET_FORMATS = ('full', 'w4', 'w4a4')
 
     @classmethod
     def arguments_parser(cls) -> ArgumentParser:
@@ -79,14 +80,14 @@ class Config:
                             help="if >0, train with sampled softmax over this many negatives "
                                  "(evaluation always uses the full softmax)")
         parser.add_argument('--transform', dest='transform', default='tanh',
-                            choices=list(cls.TRANSFORMS),
+                            choices=TRANSFORMS,
                             help="what combines a context's three vectors: one projection "
                                  "and tanh, or a gated pair of projections")
         parser.add_argument('--gate-activation', dest='gate_activation', default='silu',
-                            choices=list(cls.GATE_ACTIVATIONS),
+                            choices=GATE_ACTIVATIONS,
                             help="activation of the gate (with --transform gated)")
         parser.add_argument('--target-format', dest='target_format', default='full',
-                            choices=list(cls.TARGET_FORMATS),
+                            choices=TARGET_FORMATS,
                             help="what evaluation and prediction score names with: the target "
                                  "table in the compute dtype, its MXFP4 codes (w4), or "
                                  "those and MXFP4 code vectors (w4a4)")
@@ -330,9 +331,9 @@ class Config:
         self.verify_choices()
 
     def verify_choices(self):
-        for name, choices in (('TRANSFORM', self.TRANSFORMS),
-                              ('GATE_ACTIVATION', self.GATE_ACTIVATIONS),
-                              ('TARGET_FORMAT', self.TARGET_FORMATS)):
+        for name, choices in (('TRANSFORM', TRANSFORMS),
+                              ('GATE_ACTIVATION', GATE_ACTIVATIONS),
+                              ('TARGET_FORMAT', TARGET_FORMATS)):
             if getattr(self, name) not in choices:
                 raise ValueError('%s must be one of %s, not %r'
                                  % (name, ', '.join(choices), getattr(self, name)))

@@ -132,9 +132,7 @@ class Code2VecNetwork:
         # made again when they are next needed after the table has changed
         self._target_codes = None
         self._codes_ready = None
-        if config.TARGET_FORMAT != 'full':
-            self._target_codes = F.mxfp4_quantize(self.target_table)
-            self._targets_changed = True
+        self._targets_changed = True
 
     # ---- parameters ----
 
@@ -282,8 +280,14 @@ class Code2VecNetwork:
                      and torch.cuda.is_current_stream_capturing())
         if self._targets_changed:
             q = F.mxfp4_quantize(self.target_table)
-            self._target_codes.codes.copy_(q.codes)
-            self._target_codes.scales.copy_(q.scales)
+            if self._target_codes is None:
+                if capturing:
+                    raise RuntimeError('score once before capturing: the codes of '
+                                       'the target table have no place yet')
+                self._target_codes = q
+            else:
+                self._target_codes.codes.copy_(q.codes)
+                self._target_codes.scales.copy_(q.scales)
             if not capturing:
                 # (a capture has written nothing yet)
                 if self.device.type == 'cuda':

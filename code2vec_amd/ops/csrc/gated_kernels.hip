@@ -959,6 +959,7 @@ torch::Tensor transform_gated_fwd(torch::Tensor ctx, torch::Tensor w_oi, int64_t
   const int N = ctx.size(0), K = ctx.size(1), H = w_oi.size(1);
   auto y = torch::empty({N, H}, ctx.options());
   if (N == 0 || H == 0) return y;
+  if (K == 0) return y.zero_();          // act(0) * 0
   const Rows x = chunked_rows(ctx, K), w = chunked_rows(w_oi.view({2L * H, K}), K);
   BtArgs a{x.p, w.p, bf_mut(y), nullptr, x.ld, 0, N, H, pad8(H), pad8(K), 1.f, 0,
            nullptr};

@@ -12,7 +12,7 @@ import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
 
-from code2vec_amd.config import Config
+from code2vec_amd.config import GATE_ACTIVATIONS, Config
 from code2vec_amd.models.network import Code2VecNetwork
 from code2vec_amd.ops import functional as F
 from code2vec_amd.ops import reference as R
@@ -73,7 +73,7 @@ def autograd(net, src, pth, tgt, mask, labels, keep=None):
     return float(loss.detach()), {n: p[n].grad for n in p}
 
 
-@pytest.mark.parametrize('act', Config.GATE_ACTIVATIONS)
+@pytest.mark.parametrize('act', GATE_ACTIVATIONS)
 @pytest.mark.parametrize('keep_rate', [1.0, 0.75])
 def test_train_step_against_autograd(act, keep_rate):
     """From zero moments a step leaves a tenth of the gradient as Adam's first."""
@@ -146,7 +146,7 @@ def test_choices():
     for name in ('TRANSFORM', 'GATE_ACTIVATION', 'TARGET_FORMAT'):
         with pytest.raises(ValueError, match=name):
             make_net(**{name: 'softplus'})
-    assert set(Config.GATE_ACTIVATIONS) == set(F.GATE_ACTIVATIONS)
+    assert GATE_ACTIVATIONS == F.GATE_ACTIVATIONS
 
 
 @pytest.mark.parametrize('fmt', ['w4', 'w4a4'])
@@ -183,6 +183,11 @@ def test_answers_from_mxfp4_targets(fmt):
         other.train_step(*make_batch(s))
     net.load_state_dict(other.state_dict())
     check()
+    # asked for later
+    late = make_net()
+    late.config.TARGET_FORMAT = fmt
+    assert torch.equal(late.predict_batch(src, pth, tgt, mask, 10)[1],
+                       make_net(TARGET_FORMAT=fmt).predict_batch(src, pth, tgt, mask, 10)[1])
     # training does not look at the format
     a, b = make_net(TARGET_FORMAT=fmt), make_net()
     assert torch.equal(a.train_step(*make_batch()), b.train_step(*make_batch()))

@@ -6,7 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from code2vec_amd.config import Config  # noqa: E402
+from code2vec_amd.config import GATE_ACTIVATIONS, Config  # noqa: E402
 from code2vec_amd.models.network import Code2VecNetwork  # noqa: E402
 from code2vec_amd.ops import functional as F  # noqa: E402
 from code2vec_amd.ops import reference as R  # noqa: E402
@@ -37,7 +37,7 @@ def batch(seed, B=16, C=20, device='cuda:0'):
     return [t.to(device) for t in (src, pth, tgt, mask, labels)]
 
 
-@pytest.mark.parametrize('act', Config.GATE_ACTIVATIONS)
+@pytest.mark.parametrize('act', GATE_ACTIVATIONS)
 def test_gradients_against_the_cpu_engine(act):
     """The CPU engine in fp32 against the GPU's in bf16. From zero moments a
     step leaves a tenth of the gradient as Adam's first. On the way to one are

@@ -162,6 +162,18 @@ def test_no_rows():
     assert d_w.shape == (2, 24, 16) and (d_w == 0).all()
 
 
+@pytest.mark.parametrize('act', F.GATE_ACTIVATIONS)
+def test_no_columns(act):
+    x, w_oi, w_io, dy = make(70, 24, 16, seed=1)
+    y, kept, d_ctx, d_w = run(x[:, :0], w_oi[:, :, :0].contiguous(), w_io[:0], dy, act)
+    assert y.shape == (70, 16) and (y == 0).all()
+    assert d_ctx.shape == (70, 0) and d_w.shape == (2, 0, 16)
+    y, kept, d_ctx, d_w = run(x, w_oi[:, :0].contiguous(), w_io[:, :0].contiguous(),
+                              dy[:, :0], act)
+    assert y.shape == (70, 0) and d_w.shape == (2, 24, 0)
+    assert d_ctx.shape == (70, 24) and (d_ctx == 0).all()
+
+
 @pytest.mark.parametrize('on_device', [False, True])
 def test_dropout_mask_of_the_context(on_device):
     N, K, H = 140, 72, 80

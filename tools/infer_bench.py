@@ -11,7 +11,7 @@ import time
 
 import torch
 
-from code2vec_amd.config import Config
+from code2vec_amd.config import TARGET_FORMATS, TRANSFORMS, Config
 from code2vec_amd.models.network import Code2VecNetwork
 from code2vec_amd.serving.graph_infer import GraphCapturedPredictor
 
@@ -22,8 +22,8 @@ def main():
     ap.add_argument('--steps', type=int, default=30)
     ap.add_argument('--warmup', type=int, default=10)
     ap.add_argument('--topk', type=int, default=10)
-    ap.add_argument('--transform', choices=Config.TRANSFORMS, default='tanh')
-    ap.add_argument('--target-format', choices=Config.TARGET_FORMATS, default='full')
+    ap.add_argument('--transform', choices=TRANSFORMS, default='tanh')
+    ap.add_argument('--target-format', choices=TARGET_FORMATS, default='full')
     args = ap.parse_args()
 
     assert torch.cuda.is_available()
