@@ -97,7 +97,7 @@ __launch_bounds__(256)
 __global__ void k_mxfp4_quantize(const void* __restrict__ x, long ldx,
                                  u32* __restrict__ codes,
                                  uint8_t* __restrict__ scales, long R, int K,
-                                 int nb, int vec, int flat) {
+                                 int nb, int flat) {
   const long per_row = (long)nb * 4, total = R * per_row;
   // whole wavefronts stay in the loop together: the shuffles need all lanes
   for (long base = (long)blockIdx.x * 256; base < total;
@@ -112,9 +112,9 @@ __global__ void k_mxfp4_quantize(const void* __restrict__ x, long ldx,
     if (t < total) {
       if constexpr (F32) {
         const float* p = reinterpret_cast<const float*>(x) + r * ldx + k;
-        if (vec && k + 8 <= K_) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(p);
-          const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
+        if (k + 8 <= K_) {
+          const f32x4 a = *reinterpret_cast<const f32x4_any*>(p);
+          const f32x4 b = *reinterpret_cast<const f32x4_any*>(p + 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
         } else {
@@ -123,8 +123,8 @@ __global__ void k_mxfp4_quantize(const void* __restrict__ x, long ldx,
         }
       } else {
         const ushort* p = reinterpret_cast<const ushort*>(x) + r * ldx + k;
-        if (vec && k + 8 <= K_) {
-          const u16x8 a = *reinterpret_cast<const u16x8*>(p);
+        if (k + 8 <= K_) {
+          const u16x8 a = *reinterpret_cast<const u16x8_any*>(p);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = bf2f(a[j]);
         } else {
@@ -228,7 +228,6 @@ struct MxArgs {
   int n_tiles;                // tiles of rows of x
   int passes, passes_each;    // passes over rows of w, in all and a block
   int period;                 // rows of y this many apart lie alike on lines
-  int vec;                    // x can be read 16 bytes at a time
 };
 
 constexpr int MT = 4;         // 16-row tiles of w a wave
@@ -246,8 +245,8 @@ DEVI u32x4 x_unit(const MxArgs& p, long n, int u, u32& scale) {
     }
   } else {
     const ushort* s = p.x + n * p.ldx + u * 8;
-    if (p.vec && u * 8 + 8 <= p.K) {
-      v = *reinterpret_cast<const u32x4*>(s);
+    if (u * 8 + 8 <= p.K) {
+      v = __builtin_bit_cast(u32x4, *reinterpret_cast<const u16x8_any*>(s));
     } else {
       u16x8 e = {};
 #pragma unroll
@@ -653,15 +652,13 @@ std::vector<torch::Tensor> mxfp4_quantize(torch::Tensor x) {
   if (R == 0 || K == 0) return {codes, scales};
   auto src = K == 1 || x.stride(1) == 1 ? x : x.contiguous();
   const long ld = R == 1 ? K : src.stride(0);
-  const int vec = (ld % (f32 ? 4 : 8)) == 0 &&
-                  (reinterpret_cast<uintptr_t>(src.data_ptr()) & 15) == 0;
   // dense rows of whole blocks are one long row: no division is needed
   const int flat = K % 32 == 0 && (ld == K || R == 1);
   const int grid = grid_of(R * nb * 4, 256, 16384);
   auto* fn = f32 ? &k_mxfp4_quantize<true> : &k_mxfp4_quantize<false>;
   fn<<<grid, 256, 0, cur_stream()>>>(
       src.data_ptr(), ld, reinterpret_cast<u32*>(codes.data_ptr()),
-      scales.data_ptr<uint8_t>(), R, K, nb, vec, flat);
+      scales.data_ptr<uint8_t>(), R, K, nb, flat);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   return {codes, scales};
 }
@@ -670,17 +667,18 @@ std::vector<torch::Tensor> mxfp4_quantize(torch::Tensor x) {
 void check_mx(const torch::Tensor& codes, const torch::Tensor& scales, long K,
               const char* name) {
   const long nb = (K + 31) / 32;
-  TORCH_CHECK(codes.is_cuda() && scales.device() == codes.device(), name,
-              " must be on one GPU");
-  TORCH_CHECK(codes.scalar_type() == torch::kUInt8 &&
-              scales.scalar_type() == torch::kUInt8, name, " must be uint8");
-  TORCH_CHECK(codes.dim() == 2 && scales.dim() == 2 &&
-              codes.size(0) == scales.size(0) && scales.size(1) == nb &&
-              codes.size(1) == 16 * nb, name, " does not hold rows of ", K);
-  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous() &&
-              (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0 &&
+  TORCH_CHECK_VALUE(codes.is_cuda() && scales.device() == codes.device(), name,
+                    " must be on one GPU");
+  TORCH_CHECK_VALUE(codes.scalar_type() == torch::kUInt8 &&
+                    scales.scalar_type() == torch::kUInt8, name, " must be uint8");
+  TORCH_CHECK_VALUE(codes.dim() == 2 && scales.dim() == 2 &&
+                    codes.size(0) == scales.size(0) && scales.size(1) == nb &&
+                    codes.size(1) == 16 * nb, name, " does not hold rows of ", K);
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous(), name,
+                    " must be contiguous");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0 &&
               (reinterpret_cast<uintptr_t>(scales.data_ptr()) & 3) == 0, name,
-              " must be contiguous and start on 16 bytes, its scales on 4");
+              " must start on 16 bytes, its scales on 4");
   TORCH_CHECK(codes.size(0) < (1L << 26) && K < (1L << 20), name, " is too large");
 }
 
@@ -785,7 +783,7 @@ torch::Tensor mxfp4_matmul(torch::Tensor x,
                            int64_t K, bool f32) {
   check_mx(w_codes, w_scales, K, "w");
   const bool x4 = x_scales.has_value();
-  TORCH_CHECK(x.device() == w_codes.device(), "x and w must be on one GPU");
+  TORCH_CHECK_VALUE(x.device() == w_codes.device(), "x and w must be on one GPU");
   const Guard guard(x.device());
   torch::Tensor src = x;
   MxArgs a{};
@@ -794,13 +792,12 @@ torch::Tensor mxfp4_matmul(torch::Tensor x,
     a.xc = x.data_ptr<uint8_t>();
     a.xs = x_scales->data_ptr<uint8_t>();
   } else {
-    TORCH_CHECK(x.scalar_type() == torch::kBFloat16 && x.dim() == 2 &&
-                x.size(1) == K, "x must be a bfloat16 (N, K)");
+    TORCH_CHECK(x.scalar_type() == torch::kBFloat16, "x must be bfloat16");
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "x must be (N, ", K, ")");
     TORCH_CHECK(x.size(0) < (1L << 26), "x is too large");
     if (K > 1 && x.stride(1) != 1) src = x.contiguous();
     a.x = reinterpret_cast<const ushort*>(src.data_ptr<at::BFloat16>());
     a.ldx = x.size(0) == 1 ? K : src.stride(0);
-    a.vec = a.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
   }
   a.N = x.size(0);
   a.M = w_codes.size(0);

@@ -133,8 +133,6 @@ def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
 
 
 def _check_mxfp4(q, name: str):
-    if not isinstance(q, Mxfp4):
-        _refuse('%s must be an Mxfp4', name)
     blocks = -(-q.k // ref.MXFP4_BLOCK)
     if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8:
         _refuse('%s must hold uint8 codes and scales', name)
@@ -165,12 +163,14 @@ def mxfp4_quantize(x) -> Mxfp4:
 def mxfp4_dequantize(q: Mxfp4, dtype=torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, (N,K). They are exact in either dtype,
     bfloat16 or float32."""
-    _check_mxfp4(q, 'q')
+    if not isinstance(q, Mxfp4):
+        _refuse('q must be an Mxfp4')
     if dtype not in (torch.float32, torch.bfloat16):
         _refuse('dtype must be float32 or bfloat16, not %s', dtype)
-    if backend_for(q.codes) == 'hip':
+    if backend_for(q.codes) == 'hip':      # (which looks at q itself)
         return hip_ext(True).mxfp4_dequantize(q.codes, q.scales, q.k,
                                               dtype == torch.float32)
+    _check_mxfp4(q, 'q')
     return ref.mxfp4_dequantize(q, dtype)
 
 
@@ -182,24 +182,24 @@ def mxfp4_matmul(x, w: Mxfp4, out_dtype=torch.bfloat16) -> torch.Tensor:
     into the matrix instructions, which is exact. x an Mxfp4: both sides go
     into the scaled matrix instructions as they are. Any N, M and K. There is
     no backward: this is what a trained table answers with."""
-    _check_mxfp4(w, 'w')
+    if not isinstance(w, Mxfp4):
+        _refuse('w must be an Mxfp4')
     if out_dtype not in (torch.float32, torch.bfloat16):
         _refuse('out_dtype must be float32 or bfloat16, not %s', out_dtype)
-    scales = None
-    if isinstance(x, Mxfp4):
-        _check_mxfp4(x, 'x')
-        if x.k != w.k:
-            _refuse('x has rows of %d values, w of %d', x.k, w.k)
-        rows, scales = x.codes, x.scales
-    else:
-        if x.dim() != 2 or x.shape[1] != w.k:
-            _refuse('x must be (N,%d), not %s', w.k, tuple(x.shape))
-        rows = x
-    if rows.device != w.codes.device:
-        _refuse('x and w must be on one device')
-    if backend_for(w.codes) == 'hip':
+    both = isinstance(x, Mxfp4)
+    if both and x.k != w.k:
+        _refuse('x has rows of %d values, w of %d', x.k, w.k)
+    rows, scales = (x.codes, x.scales) if both else (x, None)
+    if backend_for(w.codes) == 'hip':      # (which looks at the rest itself)
         return hip_ext(True).mxfp4_matmul(rows, scales, w.codes, w.scales, w.k,
                                           out_dtype == torch.float32)
+    _check_mxfp4(w, 'w')
+    if both:
+        _check_mxfp4(x, 'x')
+    elif x.dim() != 2 or x.shape[1] != w.k:
+        _refuse('x must be (N,%d), not %s', w.k, tuple(x.shape))
+    if rows.device != w.codes.device:
+        _refuse('x and w must be on one device')
     return ref.mxfp4_matmul(x, w, out_dtype)
 
 

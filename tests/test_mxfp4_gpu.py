@@ -262,6 +262,18 @@ def test_refusals():
         F.mxfp4_matmul(x[:, :39], w)
     with pytest.raises(ValueError):
         F.mxfp4_quantize(x.half())
+    for bad in (F.Mxfp4(w.codes[:, :16], w.scales, 40), F.Mxfp4(w.codes, w.scales[:9], 40),
+                F.Mxfp4(w.codes, w.scales, 70), F.Mxfp4(w.codes.float(), w.scales, 40),
+                F.Mxfp4(w.codes, w.scales.cpu(), 40),
+                F.Mxfp4(w.codes.t().contiguous().t(), w.scales, 40)):
+        with pytest.raises(ValueError):
+            F.mxfp4_matmul(x, bad)
+        with pytest.raises(ValueError):
+            F.mxfp4_dequantize(bad)
+        with pytest.raises(ValueError):
+            F.mxfp4_matmul(bad, w)
+    with pytest.raises(ValueError):
+        F.mxfp4_matmul(x, w.codes)
     shifted = torch.empty(w.codes.numel() + 1, dtype=torch.uint8, device='cuda')[1:]
     with pytest.raises(RuntimeError):
         F.mxfp4_matmul(x, F.Mxfp4(shifted.view(w.codes.shape), w.scales, w.k))
