@@ -212,7 +212,7 @@ __global__ void k_mxfp4_dequantize(const u32* __restrict__ codes,
 //
 // One row by 261246 of 384: 12.0 us, bound by the reading of w (53 MB, 4.4 TB/s,
 // where bf16 weights would be 201 MB). 37 rows by 50001 of 201, y in float32:
-// 12.6 us, bound by y's broken lines (7.4 MB) and by latency.
+// 9.0 us, bound by y's broken lines (7.4 MB) and by latency.
 // ---------------------------------------------------------------------------
 
 struct MxArgs {
@@ -763,10 +763,19 @@ void launch_stream(const MxArgs& args) {
   launch_mx<&k_mxfp4_stream<X4, OUT32, R>>(a, blocks, 512, S::RING);
 }
 
+// Up to 128 rows of x go by tiles of 16 or of 64: 16 fill the chip with blocks
+// where w is short, 64 read w once. (64 and 16, y in bf16: x in bf16, K = 384, 37
+// rows by 25000 10.0 and 7.1 us, 64 by 50001 12.6 and 12.4, 128 by 50001 18.5 and
+// 23.3, 37 by 261246 26.9 and 26.2; rows of 700, which 64 at a time do not fit
+// LDS, 128 by 261246 173 and 126; x in 4 bits, 64 by 25000 7.4 and 6.4, 64 by
+// 50001 8.7 and 11.2.) More go through k_mxfp4_stream.
 template <bool X4, bool OUT32>
 void pick_mx(const MxArgs& a) {
   const int steps = (a.nb + 3) / 4;
-  if (a.N <= 16) launch_rows<X4, OUT32, 1>(a);
+  const long blocks = (long)((a.N + 15) / 16) * ((a.M + 255) / 256);
+  if (a.N <= 16 || (a.N <= 128 && (blocks <= (X4 ? 512 : 1024) ||
+                                   (!X4 && (a.N <= 48 || steps > 4)))))
+    launch_rows<X4, OUT32, 1>(a);
   else if (a.N <= 128 || a.M < 64 || steps > 6 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
     launch_rows<X4, OUT32, 4>(a);
   else if (steps <= 2) launch_stream<X4, OUT32, 2>(a);
