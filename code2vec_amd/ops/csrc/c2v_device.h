@@ -47,3 +47,14 @@ DEVI int xcd_chunked(int wg, int nwg) {
   const int xcd = wg % nxcd, orig = wg / nxcd;
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + orig;
 }
+
+// keeps a pointer in scalar registers, so that lanes add 32-bit offsets to it
+template <typename P>
+DEVI P* in_scalar(P* p) {
+  const u64 v = (u64)p;
+  u32 lo = __builtin_amdgcn_readfirstlane((u32)v);
+  u32 hi = __builtin_amdgcn_readfirstlane((u32)(v >> 32));
+  u64 w = (u64)hi << 32 | lo;
+  asm("" : "+s"(w));
+  return (P*)w;
+}

@@ -61,13 +61,6 @@ DEVI void act_both(float g, float& a, float& da) {
   }
 }
 
-// keeps a base in scalar registers, so that a load adds its 32-bit offset
-// by itself and the vector units are left to the epilogue
-DEVI const char* in_scalar(const char* p) {
-  asm("" : "+s"(p));
-  return p;
-}
-
 DEVI void to_lds16(const void* src, ushort* dst) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) u32*)src,

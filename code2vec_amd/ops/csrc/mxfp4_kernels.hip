@@ -27,17 +27,6 @@ DEVI float scale_of(u32 byte) {
   return __builtin_bit_cast(float, byte << 23);
 }
 
-// keeps a pointer in scalar registers, so that lanes add 32-bit offsets to it
-template <typename P>
-DEVI P* in_scalar(P* p) {
-  const u64 v = (u64)p;
-  u32 lo = __builtin_amdgcn_readfirstlane((u32)v);
-  u32 hi = __builtin_amdgcn_readfirstlane((u32)(v >> 32));
-  u64 w = (u64)hi << 32 | lo;
-  asm("" : "+s"(w));
-  return (P*)w;
-}
-
 DEVI u16x8 pack8(f32x4 a, f32x4 b) {
   bf16x8 v;
 #pragma unroll
