@@ -30,6 +30,11 @@ def _hip_sources(here: str):
                          'mxfp4_kernels.hip')]
 
 
+def _hip_headers(here: str):
+    return [os.path.join(here, 'csrc', name)
+            for name in ('c2v_device.h', 'c2v_launch.h')]
+
+
 def build(verbose: bool = True) -> str:
     os.environ.setdefault('PYTORCH_ROCM_ARCH', 'gfx950')
     here = os.path.dirname(os.path.abspath(__file__))
@@ -37,9 +42,7 @@ def build(verbose: bool = True) -> str:
     os.makedirs(build_dir, exist_ok=True)
     sources = _hip_sources(here)
     dest = os.path.join(here, '_c2v_hip.so')
-    headers = [os.path.join(here, 'csrc', name)
-               for name in ('c2v_device.h', 'c2v_launch.h')]
-    if _is_fresh(dest, *sources, *headers, os.path.abspath(__file__)):
+    if _is_fresh(dest, *sources, *_hip_headers(here), os.path.abspath(__file__)):
         build_reader(verbose=verbose)
         return dest
 
@@ -80,7 +83,7 @@ def build_asan(verbose: bool = True) -> str:
     sources = _hip_sources(here)
     dest = os.path.join(here, '_c2v_hip_asan.so')
     try:
-        if _is_fresh(dest, *sources):
+        if _is_fresh(dest, *sources, *_hip_headers(here)):
             return dest
         # The build runs in a SACRIFICIAL subprocess: cpp_extension.load
         # dlopens the result after building, and loading an ASAN .so into a
@@ -95,6 +98,8 @@ def build_asan(verbose: bool = True) -> str:
             "    build_directory=%r,\n"
             "    extra_cflags=['-O1', '-g'],\n"
             "    extra_cuda_cflags=['-O1', '-g', '-std=c++17',\n"
+            "                       '-Xclang', '-target-feature',\n"
+            "                       '-Xclang', '-packed-fp32-ops',\n"
             "                       '-fsanitize=address', '-shared-libsan'],\n"
             "    extra_ldflags=['-L/opt/rocm/lib/llvm/lib/clang/22/lib/linux',\n"
             "                   '-lclang_rt.asan-x86_64',\n"
