@@ -66,7 +66,7 @@ def build(verbose: bool = True) -> str:
         with_cuda=True,
     )
     built = os.path.join(build_dir, '_c2v_hip.so')
-    shutil.copy2(built, dest)
+    shutil.copy(built, dest)    # with a time of its own: it is fresh now
     build_reader(verbose=verbose)
     return dest
 
