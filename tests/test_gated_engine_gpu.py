@@ -161,3 +161,50 @@ def test_codes_made_on_another_stream():
         torch.cuda.synchronize()
         for answers in (first, second):
             check_answers(net, *answers[:3])
+
+
+def test_two_calls_at_once():
+    """The same calls on two streams, each with tensors of its own, and two captured
+    graphs of them that are replayed at once."""
+    def inputs(seed, N):
+        g = torch.Generator(device='cuda').manual_seed(seed)
+        x = torch.randn(N, 200, generator=g, device='cuda').to(torch.bfloat16)
+        w = torch.randn(2, 120, 200, generator=g, device='cuda').to(torch.bfloat16) * 0.1
+        dy = torch.randn(N, 120, generator=g, device='cuda').to(torch.bfloat16)
+        table = torch.randn(3001, 120, generator=g, device='cuda')
+        return x, w, w.permute(2, 0, 1).reshape(200, 240).contiguous(), dy, table
+
+    def run(x, w_oi, w_io, dy, table):
+        y, kept = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
+        d_ctx, d_w = F.transform_gated_bwd(x, w_io, kept, dy, 'silu')
+        q = F.mxfp4_quantize(table)
+        return y, d_ctx, d_w, F.mxfp4_matmul(y, q), F.mxfp4_matmul(F.mxfp4_quantize(y), q)
+
+    both = [inputs(1, 3000), inputs(2, 2777)]
+    want = [run(*i) for i in both]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        got = []
+        for s, i in zip(streams, both):
+            with torch.cuda.stream(s):
+                got.append(run(*i))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+    graphs, outs = [], []
+    for i in both:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(*i))
+    for _ in range(4):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))

@@ -250,6 +250,35 @@ def test_another_stream_and_a_captured_graph(K):
             assert torch.equal(a, b)
 
 
+def test_offsets_beyond_32_bits():
+    """Whole numbers and relu, exact as above: dg and du are 9 GB. dy is not zero in
+    the first and last rows alone."""
+    g = torch.Generator().manual_seed(4)
+    K = H = 384
+    N, some = 6000131, 1000
+    x = torch.zeros(some, K)
+    x[torch.arange(some), torch.randint(0, K, (some,), generator=g)] = 1.0
+    x[torch.arange(some), torch.randint(0, K, (some,), generator=g)] = 2.0
+    w = torch.randint(-2, 3, (2, K, H), generator=g).float()
+    w_oi, w_io = w.transpose(1, 2).contiguous(), w.permute(1, 0, 2).reshape(K, 2 * H)
+    b = [t.to(torch.bfloat16).cuda() for t in (x, w_oi, w_io)]
+    ctx = b[0].repeat(N // some + 1, 1)[:N]
+    dy = torch.zeros(N, H, dtype=torch.bfloat16, device='cuda')
+    ends = [0, 1, N - 2, N - 1]
+    dy[ends, torch.randint(0, H, (4,), generator=g).cuda()] = 1.0
+    y, kept = F.transform_gated_fwd(ctx, b[1], 'relu', save=True)
+    yr = R.transform_gated_fwd(x, w_oi, 'relu')
+    rows = torch.arange(N - 3000, N)
+    assert torch.equal(y[N - 3000:].cpu().float(), yr[rows % some])
+    assert torch.equal(y[:some].cpu().float(), yr)
+    d_ctx, d_w = F.transform_gated_bwd(ctx, b[2], kept, dy, 'relu')
+    xe = x[torch.tensor(ends) % some]
+    dxr, dwr = R.transform_gated_bwd(xe, w_io, w_oi, dy[ends].cpu().float(), 'relu')
+    assert torch.equal(d_ctx[ends].cpu().float(), dxr)
+    assert not d_ctx[2:N - 2].any()
+    assert torch.equal(d_w.cpu().float(), dwr)
+
+
 def test_refusals():
     x, w_oi, w_io, dy = (t.cuda() for t in make(10, 16, 8, seed=1))
     with pytest.raises(ValueError):
