@@ -9,6 +9,7 @@ import time
 
 import torch
 
+from code2vec_amd.ops import functional as F
 from code2vec_amd.ops import hip_ext
 
 B, C, d, D, V = 1024, 200, 128, 384, 261246
@@ -49,8 +50,22 @@ def main():
     timeit('gemm_bt (our MFMA, no tanh)', lambda: ext.gemm_bt_bf16(ctx, w_oi))
     timeit('torch.matmul same shape', lambda: ctx @ w_oi.t())
 
+    gw_oi = torch.randn(2, D, D, device=dev).to(torch.bfloat16) * 0.05
+    gw_io = gw_oi.permute(2, 0, 1).reshape(D, 2 * D).contiguous()
+    d_y = torch.randn(N, D, device=dev).to(torch.bfloat16)
+    timeit('gated transform fwd', lambda: F.transform_gated_fwd(ctx, gw_oi))
+    timeit('gated transform bwd',
+           lambda: F.transform_gated_bwd(ctx, gw_io, gw_oi, d_y))
+
     timeit('logits hipBLASLt', lambda: code @ shadow.t())
     timeit('logits our gemm_bt', lambda: ext.gemm_bt_bf16(code, shadow))
+    targets = F.mxfp4_quantize(shadow)
+    timeit('MXFP4 of the target table', lambda: F.mxfp4_quantize(shadow))
+    timeit('logits MXFP4 targets', lambda: F.mxfp4_matmul(code, targets))
+    timeit('logits MXFP4 both sides',
+           lambda: F.mxfp4_matmul(F.mxfp4_quantize(code), targets))
+    timeit('logits MXFP4 targets, one row', lambda: F.mxfp4_matmul(code[:1], targets))
+    timeit('logits hipBLASLt, one row', lambda: code[:1] @ shadow.t())
 
     dl = torch.randn(B, V, device=dev).to(torch.bfloat16)
     timeit('d_code hipBLASLt', lambda: dl @ shadow)
