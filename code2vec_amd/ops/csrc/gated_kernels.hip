@@ -890,18 +890,26 @@ void rows_gemm(const BtArgs& a) {
 
 // dW by tiles of CA columns of dgu by CB of x, the rows in S parts. A part
 // more than fills the chip costs a whole round, and every part costs the
-// writing and reading of its sums.
+// writing and reading of its sums. Fitted like the rates of rows_gemm; what is
+// chosen is the best of these, or within 13% of it, at ten sizes. In us, each
+// tile with its best number of parts, their sum included:
+//   rows  K to H       256x128   128x128   64x64
+//    512  192 to 192      11.8       9.7     8.3
+//   2000 1000 to 1000     30.0      27.0    29.5
+//   7000 1250 to 720      52.1      50.8    67.6
+//  14351 1440 to 1440      169       171     226
+// 100000  200 to 200       181        61      68
+// 204800  384 to 384       187       192     272
 struct DwPlan { double us; int S; };
 
-DwPlan plan_dw(long N, long C2, long K, int CA, int CB, double slots, double alone,
-               double full) {
+DwPlan plan_dw(long N, long C2, long K, int CA, int CB, double slots, double fixed,
+               double alone, double full) {
   const double tiles = std::ceil(C2 / (double)CA) * std::ceil(K / (double)CB);
   DwPlan best{1e30, 1};
   for (int S = 1; S <= 64 && (S == 1 || N / S >= 64); ++S) {
-    const double load = std::min(1.0, tiles * S / slots);
-    const double us = std::ceil(tiles * S / slots) *
-                          (3 + std::ceil(N / (double)S / TN_ROWS) * (alone + (full - alone) * load)) +
-                      (S > 1 ? 3 + S * (double)(C2 * K) * 8 / 5e6 : 0);
+    const double us = launch_us(tiles * S, slots, std::ceil(N / (double)S / TN_ROWS),
+                                alone, full, fixed) +
+                      (S > 1 ? 4.5 + S * (double)(C2 * K) * 8 / 5e6 : 0);
     if (us < best.us) best = {us, S};
   }
   return best;
@@ -1012,10 +1020,13 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   rows_gemm<PLAIN, SILU>(a);
 
   auto d_w = torch::empty({2, K, H}, ctx.options());
-  const DwPlan large = plan_dw(N, 2L * Hp, K, 256, 128, 512, 0.6, 1.3);
-  const DwPlan small = plan_dw(N, 2L * Hp, K, 64, 64, 1024, 0.3, 0.6);
-  if (large.us <= small.us)
+  const DwPlan large = plan_dw(N, 2L * Hp, K, 256, 128, 512, 4.25, 0.86, 0.9);
+  const DwPlan middle = plan_dw(N, 2L * Hp, K, 128, 128, 768, 1.8, 0.7, 0.76);
+  const DwPlan small = plan_dw(N, 2L * Hp, K, 64, 64, 1536, 1.0, 0.5, 0.75);
+  if (large.us <= std::min(middle.us, small.us))
     launch_dw<2, 2, 8, 4>(d_w, bf_ptr(dgu), x, N, K, H, Hp, large.S);
+  else if (middle.us <= small.us)
+    launch_dw<2, 2, 4, 4>(d_w, bf_ptr(dgu), x, N, K, H, Hp, middle.S);
   else
     launch_dw<2, 2, 2, 2>(d_w, bf_ptr(dgu), x, N, K, H, Hp, small.S);
   return {d_ctx, d_w};
