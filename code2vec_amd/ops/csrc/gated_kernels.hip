@@ -456,7 +456,9 @@ __global__ void k_rows_gemm(BtArgs p) {
       multiply(f);
       multiply(g);
       flip();
+      // every wave has what it read of the buffer that is filled next
       asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt alone
       block_barrier();
       ask(EPI == DGATED);
     }
