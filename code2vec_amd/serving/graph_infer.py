@@ -20,6 +20,8 @@ class GraphCapturedPredictor:
                  warmup: int = 3):
         assert network.device.type == 'cuda', 'graph capture needs a GPU'
         self.net = network
+        # what is captured stays as it is, whatever the configuration becomes
+        self.from_codes = network.config.TARGET_FORMAT != 'full'
         self.B = batch_size
         self.k = top_k
         C = network.config.MAX_CONTEXTS
@@ -49,10 +51,10 @@ class GraphCapturedPredictor:
                                   out_dtype=net.compute_dtype)
         comb, _ = net.transform(ctx)
         code, alpha = F.attention_fwd(comb.reshape(B, C, D), net.a_c, self.mask)
-        if net.config.TARGET_FORMAT == 'full':
-            logits = code.to(net.compute_dtype) @ net.target_shadow.t()
-        else:
+        if self.from_codes:
             logits = net.logits(code)
+        else:
+            logits = code.to(net.compute_dtype) @ net.target_shadow.t()
         scores, indices = F.topk(logits, k=self.k)
         return indices, scores, code
 
@@ -70,7 +72,7 @@ class GraphCapturedPredictor:
         if n < self.B:
             self.mask[n:, :].zero_()
             self.mask[n:, 0] = 1.0  # keep padded rows numerically benign
-        if self.net.config.TARGET_FORMAT != 'full':
+        if self.from_codes:
             self.net.target_codes()   # the replay reads them as they are
         self.graph.replay()
         idx, scores, code = self.out

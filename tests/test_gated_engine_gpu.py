@@ -140,6 +140,15 @@ def test_train_then_answer(fmt, B):
         step.step(*batch(10 + s))
     after = check(one)
     assert not torch.equal(before, after)
+    # a captured predictor goes on when others answer from the full table
+    net.config.TARGET_FORMAT = 'full'
+    full = GraphCapturedPredictor(net, B, 10)
+    step.step(*batch(20))
+    idx, scores, code = full.predict(src, pth, tgt, mask)
+    assert torch.equal(scores, F.topk(code.to(torch.bfloat16) @ net.target_shadow.t(), k=10)[0])
+    one.predict(src, pth, tgt, mask)
+    net.config.TARGET_FORMAT = fmt
+    check_answers(net, *one.out)
     # the loss of an evaluation
     loss = net.eval_batch(src, pth, tgt, mask, labels, 10)[4]
     st = net.forward(src, pth, tgt, mask, training=False)
