@@ -518,11 +518,13 @@ __global__ void k_mxfp4_stream(MxArgs p) {
   for (int k = -1; k < 2; ++k) fetch(pass0 + k);
 
   // Row t*4 of this lane in a pass: behind the tile's first row, or in the
-  // tile before it. A step may have fewer than four blocks: the others repeat
-  // the last.
+  // tile before it. A row's last step may have fewer than four blocks: the
+  // others repeat the last, under a scale of one, because what lies behind a row
+  // is another row, whose NaN would outlive the zeros that x has there.
   const int row_in = (l16 >> 2) * (4 * MT) + (l16 & 3) - shift;
-  const int left = nb - (R - 1) * 4;               // may be below one for R == 2
-  const int q_end = min(q, max(left, 1) - 1);
+  const int s_end = R == 2 && nb <= 4 ? 0 : R - 1;   // (other R: nb > 4 * (R - 1))
+  const int left = nb - s_end * 4;
+  const int q_end = min(q, left - 1);
 
   const int end = (p.M - 1) / 64;                  // the table's last tile
   const int odd = (int)(((long)p.M * nb) & 3);
@@ -553,12 +555,12 @@ __global__ void k_mxfp4_stream(MxArgs p) {
       const uint8_t* s_row = sm_scales + at * 4 * R + in * nb;
 #pragma unroll
       for (int s = 0; s < R; ++s) {
-        if (R == 2 && s * 4 >= nb) break;
-        const int at_q = s == R - 1 ? q_end : q;
+        if (R == 2 && s > s_end) break;
+        const int at_q = s == s_end ? q_end : q;
         const u32x4 c = *reinterpret_cast<const u32x4*>(
             c_row + s * 64 + (at_q ^ key(in)) * 16);
         u32 sc = s_row[s * 4 + at_q];
-        if (s == R - 1 && q >= left) sc = 127;
+        if (s == s_end && q >= left) sc = 127;
         if constexpr (X4) {
           const i32x8 wf = {(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
 #pragma unroll

@@ -189,6 +189,50 @@ def test_scales_at_both_ends_and_nan_blocks():
         assert v[:4, tame].isfinite().all() and v[5:, tame].isfinite().all()
 
 
+@pytest.mark.parametrize('K', [20, 32, 50, 96, 128, 160, 270, 385])
+@pytest.mark.parametrize('N', [130, 300])
+def test_nan_blocks_stay_in_their_columns(N, K):
+    """More rows than the kernel for few of them takes. Rows of the table with a NaN
+    block and rows whose scales leave bfloat16 (4 * 2^126 and more), the table's
+    first, last and those at a tile's border among them: only their own columns
+    may see them."""
+    M = 333
+    bad, nan = [0, 5, 64, 100, 127, 200, M - 1], [5, 64, 200, M - 1]
+    w = R.mxfp4_quantize(rows(M, K, 3))
+    blocks = w.scales.shape[1]
+    w.scales[0, -1], w.scales[100, 0], w.scales[127] = 254, 253, 253
+    for k, m in enumerate(nan):
+        w.scales[m, k % blocks] = 255
+    x = rows(N, K, 4, BF)
+    xq = R.mxfp4_quantize(x)
+    tame = torch.ones(M, dtype=torch.bool)
+    tame[bad] = False
+    for out in (F32, BF):
+        for a, ag in ((x, x.cuda()), (xq, on_gpu(xq))):
+            y = F.mxfp4_matmul(ag, on_gpu(w), out)
+            assert y[:, nan].isnan().all()
+            assert y.cpu()[:, tame].isfinite().all()
+            check_product(a, F.Mxfp4(w.codes[tame], w.scales[tame], K), y[:, tame.cuda()], out)
+
+
+def test_nan_blocks_of_a_table_beyond_the_caches():
+    """The same where rows of y are taken that lie alike on cache lines. Whole
+    numbers: each clean column is exact."""
+    g = torch.Generator(device='cuda').manual_seed(2)
+    N, M, K = 2040, 50001, 70
+    x = torch.randint(-4, 5, (N, K), generator=g, device='cuda').float()
+    w = torch.randint(-4, 5, (M, K), generator=g, device='cuda').float()
+    nan = torch.arange(17, M, 211, device='cuda')
+    want = x @ w.t()
+    want[:, nan] = float('nan')
+    wq = F.mxfp4_quantize(w)
+    wq.scales[nan, 0] = 255
+    for a in (x.to(BF), F.mxfp4_quantize(x)):
+        y = F.mxfp4_matmul(a, wq, BF)
+        assert torch.equal(y.isnan(), want.isnan())
+        assert torch.equal(y.nan_to_num(7.0), want.to(BF).nan_to_num(7.0))
+
+
 def test_what_fills_up_a_row_does_not_count():
     """Codes behind K are the table owner's: whatever they are, no result changes."""
     w = F.mxfp4_quantize(rows(200, 40, 1).cuda())
