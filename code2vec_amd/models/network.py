@@ -496,8 +496,8 @@ class Code2VecNetwork:
             d_ctx, d_w = F.transform_gated_bwd(
                 st.ctx, self.w_io, st.kept, d_comb.reshape(B * C, D),
                 cfg.GATE_ACTIVATION, cfg.DROPOUT_KEEP_RATE, st.seed,
-                seed_t=st.seed_t)
-            d_w = d_w.float()   # ranks and Adam add in fp32
+                seed_t=st.seed_t,
+                dw_dtype=torch.float32)   # ranks and Adam add in fp32
         else:
             # attention backward emits dL/dz directly (tanh' fused into its
             # d_comb write); the dX GEMM applies the dropout mask in its epilogue

@@ -611,13 +611,20 @@ DEVI bf16x8 tr_read(const ushort* tile, int stride, int c0, int l16, int q) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// d_w is float32 or bf16: one of d_w32 and d_w is null
+DEVI void put_sums(float* to, const float* v, int h, int H) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (h + j < H) to[j] = v[j];
+}
+
 template <int WA, int WB, int AT, int BT>
 __launch_bounds__(WA * WB * 64, 2)
 __global__ void k_dw_part(const ushort* __restrict__ dgu,
                           const ushort* __restrict__ x, long ldx,
                           float* __restrict__ part, ushort* __restrict__ d_w,
-                          int N, int C2, int K, int K8, int H, int rows_each,
-                          int tiles) {
+                          float* __restrict__ d_w32, int N, int C2, int K, int K8,
+                          int H, int rows_each, int tiles) {
   constexpr int T = WA * WB * 64;
   constexpr int CA = WA * AT * 16;     // columns of dgu a block
   constexpr int CB = WB * BT * 16;     // columns of x a block
@@ -723,18 +730,20 @@ __global__ void k_dw_part(const ushort* __restrict__ dgu,
       } else {
         const int g = c >= C2 / 2, h = c - g * (C2 / 2);
         const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        put<1>(d_w + ((long)g * K + k) * H + h, v, h, H);
+        const long at = ((long)g * K + k) * H + h;
+        if (d_w32) put_sums(d_w32 + at, v, h, H);
+        else put<1>(d_w + at, v, h, H);
       }
     }
   }
 }
 
-// d_w (2, K, H) bf16 from the parts (S, K, 2, Hp). 56 parts of 384 by 768 (66 MB):
+// d_w (2, K, H) from the parts (S, K, 2, Hp). 56 parts of 384 by 768 (66 MB):
 // 11.9 us, and 17.7 with fewer loads on their way at a time.
 __launch_bounds__(256)
 __global__ void k_dw_reduce(const float* __restrict__ part,
-                            ushort* __restrict__ d_w, int S, int K, int H,
-                            int Hp) {
+                            ushort* __restrict__ d_w, float* __restrict__ d_w32,
+                            int S, int K, int H, int Hp) {
   const long quads = (long)K * 2 * Hp / 4;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= quads) return;
@@ -745,11 +754,10 @@ __global__ void k_dw_reduce(const float* __restrict__ part,
   const long k = i * 4 / (2 * Hp);
   const int c = (int)(i * 4 % (2 * Hp));
   const int g = c / Hp, h = c % Hp;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (h + j < H)
-      d_w[((long)g * K + k) * H + h + j] =
-          __builtin_bit_cast(ushort, (__bf16)sum[j]);
+  const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+  const long at = ((long)g * K + k) * H + h;
+  if (d_w32) put_sums(d_w32 + at, v, h, H);
+  else put<1>(d_w + at, v, h, H);
 }
 
 // (R, C) with rows ld apart -> (R, Cp), the columns behind C zero
@@ -926,6 +934,9 @@ void launch_dw(const torch::Tensor& d_w, const ushort* dgu, const Rows& x, long 
   constexpr size_t bytes = 3ul * TN_ROWS * (CA + CB) * sizeof(ushort);
   const int tiles = (2 * Hp + CA - 1) / CA * ((K + CB - 1) / CB);
   const int rows_each = (int)(((N + S - 1) / S + TN_ROWS - 1) / TN_ROWS * TN_ROWS);
+  const bool f32 = d_w.scalar_type() == torch::kFloat32;
+  ushort* dw16 = f32 ? nullptr : bf_mut(d_w);
+  float* dw32 = f32 ? d_w.data_ptr<float>() : nullptr;
   torch::Tensor part;
   if (S > 1)
     part = torch::empty({S, K, 2L * Hp}, d_w.options().dtype(torch::kFloat32));
@@ -933,13 +944,13 @@ void launch_dw(const torch::Tensor& d_w, const ushort* dgu, const Rows& x, long 
   static std::atomic<u64> ready{0};
   allow_lds(fn, bytes, ready);
   fn<<<tiles * S, WA * WB * 64, bytes, cur_stream()>>>(
-      dgu, x.p, x.ld, S > 1 ? part.data_ptr<float>() : nullptr, bf_mut(d_w), (int)N,
+      dgu, x.p, x.ld, S > 1 ? part.data_ptr<float>() : nullptr, dw16, dw32, (int)N,
       2 * Hp, K, pad8(K), H, rows_each, tiles);
   C10_HIP_KERNEL_LAUNCH_CHECK();
   if (S == 1) return;
   const long quads = (long)K * 2 * Hp / 4;
   k_dw_reduce<<<(int)((quads + 255) / 256), 256, 0, cur_stream()>>>(
-      part.data_ptr<float>(), bf_mut(d_w), S, K, H, Hp);
+      part.data_ptr<float>(), dw16, dw32, S, K, H, Hp);
   C10_HIP_KERNEL_LAUNCH_CHECK();
 }
 
@@ -972,13 +983,14 @@ torch::Tensor transform_gated_fwd(torch::Tensor ctx, torch::Tensor w_oi, int64_t
   return y;
 }
 
-// d_ctx (N,K) and d_w (2,K,H)
+// d_ctx (N,K) and d_w (2,K,H), bf16 or, as it was summed, float32
 std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
                                                torch::Tensor w_io,
                                                torch::Tensor w_oi,
                                                torch::Tensor d_y, int64_t act,
                                                double keep_prob, int64_t seed,
-                                               c10::optional<torch::Tensor> seed_t) {
+                                               c10::optional<torch::Tensor> seed_t,
+                                               bool dw_f32) {
   check_bf16(ctx, "ctx", 2, ctx);
   check_bf16(w_io, "w_io", 2, ctx);
   check_bf16(d_y, "d_y", 2, ctx);
@@ -1000,8 +1012,9 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
   }
   const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(ctx.device());
   auto d_ctx = torch::empty({N, K}, ctx.options());
-  if (N == 0 || H == 0 || K == 0)
-    return {d_ctx.zero_(), torch::zeros({2, K, H}, ctx.options())};
+  auto d_w = torch::empty({2, K, H}, ctx.options().dtype(
+      dw_f32 ? torch::kFloat32 : torch::kBFloat16));
+  if (N == 0 || H == 0 || K == 0) return {d_ctx.zero_(), d_w.zero_()};
 
   const Rows x = chunked_rows(ctx, K);
   auto dgu = torch::empty({N, 2, Hp}, ctx.options());
@@ -1023,7 +1036,6 @@ std::vector<torch::Tensor> transform_gated_bwd(torch::Tensor ctx,
            pad8(K), 2 * Hp, (float)keep_prob, (u64)seed, seed_ptr};
   rows_gemm<PLAIN, SILU>(a);
 
-  auto d_w = torch::empty({2, K, H}, ctx.options());
   const DwPlan large = plan_dw(N, 2L * Hp, K, 256, 128, 512, 4.25, 0.86, 0.9);
   const DwPlan middle = plan_dw(N, 2L * Hp, K, 128, 128, 768, 1.8, 0.7, 0.76);
   const DwPlan small = plan_dw(N, 2L * Hp, K, 64, 64, 1536, 1.0, 0.5, 0.75);

@@ -97,12 +97,14 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
 
 
 def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
-                        keep_prob: float = 1.0, seed: int = 0, seed_t=None
-                        ) -> Tuple[torch.Tensor, torch.Tensor]:
+                        keep_prob: float = 1.0, seed: int = 0, seed_t=None,
+                        dw_dtype=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Backward of the gated transform. ctx as in the forward; w_io (K,2H)
     the same weights in-major, gate columns then up columns; kept what the
     forward kept; d_y (N,H). Returns (d_ctx (N,K), d_w (2,K,H)), in ctx's
-    type. With keep_prob < 1 d_ctx goes through the keep mask of the dropout
+    type; d_w in dw_dtype if given, that type or float32, in which it is summed:
+    for an optimizer with float32 masters, and for ranks that add theirs up. With
+    keep_prob < 1 d_ctx goes through the keep mask of the dropout
     that made ctx (gather_concat_fwd with the same seed) on its way out."""
     if activation not in GATE_ACTIVATIONS:
         _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
@@ -119,12 +121,14 @@ def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
             _refuse('ctx, w_io, kept and d_y must have one type and one device')
     if not 0.0 < keep_prob <= 1.0:
         _refuse('keep_prob must be in (0, 1]')
+    if dw_dtype not in (None, ctx.dtype, torch.float32):
+        _refuse("dw_dtype must be float32 or ctx's type, not %s", dw_dtype)
     if backend_for(ctx) == 'hip':
         d_ctx, d_w = hip_ext(True).transform_gated_bwd(
             ctx, w_io, kept, d_y, GATE_ACTIVATIONS.index(activation), keep_prob,
-            seed, seed_t)
+            seed, seed_t, dw_dtype == torch.float32)
         return d_ctx, d_w
-    d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, kept, d_y, activation)
+    d_ctx, d_w = ref.transform_gated_bwd(ctx, w_io, kept, d_y, activation, dw_dtype)
     if keep_prob < 1.0:
         if seed_t is not None:
             seed = int(seed_t.item())

@@ -133,10 +133,10 @@ def transform_gated_fwd(ctx: torch.Tensor, w_oi: torch.Tensor,
 
 
 def transform_gated_bwd(ctx: torch.Tensor, w_io: torch.Tensor, w_oi: torch.Tensor,
-                        d_y: torch.Tensor, activation: str
+                        d_y: torch.Tensor, activation: str, dw_dtype=None
                         ) -> Tuple[torch.Tensor, torch.Tensor]:
     """w_io (K,2H) and w_oi (2,H,K), the same weights: d_ctx (N,K) and d_w
-    (2,K,H), in ctx's type. dg = dy u act'(g); du = dy act(g); d_ctx =
+    (2,K,H), in ctx's type or d_w in dw_dtype. dg = dy u act'(g); du = dy act(g); d_ctx =
     [dg|du] w_io^T; d_w = ctx^T [dg|du]."""
     H = d_y.shape[1]
     x, w, dy = _wide(ctx), _wide(w_oi), _wide(d_y)
@@ -146,7 +146,7 @@ def transform_gated_bwd(ctx: torch.Tensor, w_io: torch.Tensor, w_oi: torch.Tenso
     d_ctx = dgu @ _wide(w_io).t()
     d_w = x.t() @ dgu                                          # (K, 2H)
     d_w = d_w.reshape(ctx.shape[1], 2, H).permute(1, 0, 2).contiguous()
-    return d_ctx.to(ctx.dtype), d_w.to(ctx.dtype)
+    return d_ctx.to(ctx.dtype), d_w.to(dw_dtype or ctx.dtype)
 
 
 # ---------------------------------------------------------------------------

@@ -13,7 +13,7 @@ import torch.distributed as dist
 import torch.multiprocessing as mp
 
 from code2vec_amd.config import GATE_ACTIVATIONS, Config
-from code2vec_amd.models.network import Code2VecNetwork
+from code2vec_amd.models.network import Code2VecNetwork, NullReducer
 from code2vec_amd.ops import functional as F
 from code2vec_amd.ops import reference as R
 
@@ -106,6 +106,35 @@ def test_the_tanh_engine_is_what_it_was():
                      a.tok_table[tgt.long()]], dim=-1).reshape(B * C, -1)
     assert torch.allclose(st.comb, torch.tanh(ctx @ a.w), atol=1e-5)
     assert st.kept is None
+
+
+def test_weight_gradient_is_not_rounded(monkeypatch):
+    """In bf16, too, ranks and Adam get the weights' gradient as it was summed, in
+    32 bits: next to all of the sums have more than bf16's 8."""
+    net = make_net(COMPUTE_DTYPE='bf16')
+    seen = {}
+
+    class Watch:
+        def __getattr__(self, name):
+            return getattr(NullReducer(), name)
+
+        def allreduce_dense(self, name, grad):
+            seen[name] = grad.clone()
+
+    calls = []
+    inner = F.transform_gated_bwd
+    monkeypatch.setattr(F, 'transform_gated_bwd',
+                        lambda *a, **kw: calls.append([t.clone() for t in a[:4]])
+                        or inner(*a, **kw))
+    net.train_step(*make_batch(), reducer=Watch())
+    d_w = seen['w']
+    assert d_w.dtype == torch.float32
+    ctx, w_io, kept, d_y = calls[0]
+    want = R.transform_gated_bwd(ctx.float(), w_io.float(), kept.float(), d_y.float(),
+                                 'silu')[1]
+    assert torch.equal(d_w, want)
+    assert (d_w != d_w.to(torch.bfloat16).float()).float().mean() > 0.9
+    assert torch.equal(net._adam_m['w'], d_w.mul(1 - net.config.ADAM_BETA1))
 
 
 def test_forward_for_answers_keeps_nothing():

@@ -112,6 +112,32 @@ def test_sizes(N, K, H):
     check_bwd(x, w_io, dy, 'silu', d_ctx, d_w)
 
 
+@pytest.mark.parametrize('N,K,H', [
+    (1, 384, 384), (3, 1, 1), (200, 384, 384), (33, 99, 101), (300, 31, 7), (513, 390, 391),
+    (5000, 192, 192), (4097, 136, 520), (20001, 390, 250)])
+def test_weight_gradient_in_float32(N, K, H):
+    """float32 on request, as it is summed: rounded it is the default's, bit by
+    bit. Of small whole numbers and relu each value on the way has a bfloat16
+    and each sum is below 2^24, so that the sums are exact."""
+    x, w_oi, w_io, dy = make(N, K, H, seed=N + K + H)
+    g = torch.Generator().manual_seed(N)
+    whole = torch.zeros(N, K)
+    for _ in range(2):
+        whole[torch.arange(N), torch.randint(0, K, (N,), generator=g)] = 1.0
+    w = torch.randint(0, 3, (2, K, H), generator=g).float()
+    sums = (whole, w.transpose(1, 2).contiguous(), w.permute(1, 0, 2).reshape(K, 2 * H),
+            torch.randint(0, 4, (N, H), generator=g).float())
+    want = R.transform_gated_bwd(*(sums[i].double() for i in (0, 2, 1, 3)), 'relu')[1]
+    for inputs, act in (((x, w_oi, w_io, dy), 'silu'), (sums, 'relu')):
+        inputs = [t.to(torch.bfloat16).cuda() for t in inputs]
+        _, kept, d_ctx, d_w = run(*inputs, act)
+        again, d_w32 = F.transform_gated_bwd(inputs[0], inputs[2], kept, inputs[3], act,
+                                             dw_dtype=torch.float32)
+        assert d_w32.dtype == torch.float32 and d_w.dtype == torch.bfloat16
+        assert torch.equal(again, d_ctx) and torch.equal(d_w32.to(torch.bfloat16), d_w)
+    assert torch.equal(d_w32.cpu().double(), want)
+
+
 @pytest.mark.parametrize('K', [40, 904])
 def test_whole_numbers_are_exact(K):
     """Small whole numbers and relu: every value on the way has a bfloat16."""

@@ -75,6 +75,23 @@ def test_gated_dropout_mask_is_the_gathers():
     assert torch.equal(got, F.gather_concat_bwd(plain, 0.75, 77, True))
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32, torch.float64])
+def test_gated_weight_gradient_in_float32(dtype):
+    """float32 on request, from the same sums: rounded they are the default's."""
+    x, w_oi, w_io, dy = gated_inputs(N=9, K=16, H=8, seed=3, dtype=dtype)
+    _, kept = F.transform_gated_fwd(x, w_oi, save=True)
+    d_ctx, d_w = F.transform_gated_bwd(x, w_io, kept, dy)
+    again, d_w32 = F.transform_gated_bwd(x, w_io, kept, dy, dw_dtype=torch.float32)
+    same = F.transform_gated_bwd(x, w_io, kept, dy, dw_dtype=dtype)[1]
+    assert d_w.dtype == same.dtype == dtype and d_w32.dtype == torch.float32
+    assert torch.equal(d_ctx, again) and torch.equal(d_w, same)
+    small = dtype if dtype == torch.bfloat16 else torch.float32
+    assert torch.equal(d_w32.to(small), d_w.to(small))
+    for bad in (torch.float16, torch.int32):
+        with pytest.raises(ValueError, match='dw_dtype'):
+            F.transform_gated_bwd(x, w_io, kept, dy, dw_dtype=bad)
+
+
 def test_gated_refusals():
     x, w_oi, w_io, dy = gated_inputs()
     y, kept = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
