@@ -667,9 +667,8 @@ void check_mx(const torch::Tensor& codes, const torch::Tensor& scales, long K,
                     codes.size(1) == 16 * nb, name, " does not hold rows of ", K);
   TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous(), name,
                     " must be contiguous");
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0 &&
-              (reinterpret_cast<uintptr_t>(scales.data_ptr()) & 3) == 0, name,
-              " must start on 16 bytes, its scales on 4");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) == 0, name,
+              " must start on 16 bytes");
   TORCH_CHECK(codes.size(0) < (1L << 26) && K < (1L << 20), name, " is too large");
 }
 
@@ -754,6 +753,8 @@ void launch_stream(const MxArgs& args) {
   launch_mx<&k_mxfp4_stream<X4, OUT32, R>>(a, blocks, 512, S::RING);
 }
 
+constexpr int FEW = 128;
+
 // Up to 128 rows of x go by tiles of 16 or of 64: 16 fill the chip with blocks
 // where w is short, 64 read w once. (64 and 16, y in bf16: x in bf16, K = 384, 37
 // rows by 25000 10.0 and 7.1 us, 64 by 50001 12.6 and 12.4, 128 by 50001 18.5 and
@@ -764,10 +765,10 @@ template <bool X4, bool OUT32>
 void pick_mx(const MxArgs& a) {
   const int steps = (a.nb + 3) / 4;
   const long blocks = (long)((a.N + 15) / 16) * ((a.M + 255) / 256);
-  if (a.N <= 16 || (a.N <= 128 && (blocks <= (X4 ? 512 : 1024) ||
+  if (a.N <= 16 || (a.N <= FEW && (blocks <= (X4 ? 512 : 1024) ||
                                    (!X4 && (a.N <= 48 || steps > 4)))))
     launch_rows<X4, OUT32, 1>(a);
-  else if (a.N <= 128 || a.M < 64 || steps > 6 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
+  else if (a.N <= FEW || a.M < 64 || steps > 6 || 64l * a.M * (OUT32 ? 4 : 2) >= (1L << 32))
     launch_rows<X4, OUT32, 4>(a);
   else if (steps <= 2) launch_stream<X4, OUT32, 2>(a);
   else if (steps == 3) launch_stream<X4, OUT32, 3>(a);
@@ -804,6 +805,10 @@ torch::Tensor mxfp4_matmul(torch::Tensor x,
   a.K = K;
   a.nb = w_scales.size(1);
   a.wc = w_codes.data_ptr<uint8_t>();
+  // k_mxfp4_stream reads scales as words: those of some rows of a table may start
+  // on any byte, and are copied (a 17th of the table)
+  if (a.N > FEW && (reinterpret_cast<uintptr_t>(w_scales.data_ptr()) & 3))
+    w_scales = w_scales.clone();
   a.ws = w_scales.data_ptr<uint8_t>();
   auto y = torch::empty({a.N, a.M}, w_codes.options().dtype(
       f32 ? torch::kFloat32 : torch::kBFloat16));

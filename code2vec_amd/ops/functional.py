@@ -184,8 +184,10 @@ def mxfp4_matmul(x, w: Mxfp4, out_dtype=torch.bfloat16) -> torch.Tensor:
 
     x a bfloat16 tensor: only the weights are in 4 bits, decoded on the way
     into the matrix instructions, which is exact. x an Mxfp4: both sides go
-    into the scaled matrix instructions as they are. Any N, M and K. There is
-    no backward: this is what a trained table answers with."""
+    into the scaled matrix instructions as they are. Any N, M and K; either Mxfp4
+    may be some rows of another (on the GPU its codes start on 16 bytes, as
+    every row's do). There is no backward: this is what a trained table answers
+    with."""
     if not isinstance(w, Mxfp4):
         _refuse('w must be an Mxfp4')
     if out_dtype not in (torch.float32, torch.bfloat16):

@@ -244,6 +244,30 @@ def test_what_fills_up_a_row_does_not_count():
     assert torch.equal(F.mxfp4_matmul(F.mxfp4_quantize(x), w, F32), want4)
 
 
+@pytest.mark.parametrize('K', [20, 96, 130, 700])
+@pytest.mark.parametrize('N', [1, 40, 200])
+def test_rows_of_a_table(N, K):
+    """Some rows of a table, and of quantised rows, are as good as a copy of them: an
+    odd number of blocks a row lets their scales start on any byte."""
+    w, x = (on_gpu(R.mxfp4_quantize(rows(n, K, n))) for n in (700, N + 3))
+
+    def part(q, at, n):
+        return F.Mxfp4(q.codes[at:at + n], q.scales[at:at + n], K)
+
+    def copy(q):
+        return F.Mxfp4(q.codes.clone(), q.scales.clone(), K)
+
+    rows_bf = rows(N, K, 9, BF).cuda()
+    for at in (1, 2, 3):
+        wp, xp = part(w, at, 690), part(x, at, N)
+        for out in (F32, BF):
+            assert torch.equal(F.mxfp4_dequantize(wp, out), F.mxfp4_dequantize(copy(wp), out))
+            assert torch.equal(F.mxfp4_matmul(rows_bf, wp, out),
+                               F.mxfp4_matmul(rows_bf, copy(wp), out))
+            assert torch.equal(F.mxfp4_matmul(xp, wp, out),
+                               F.mxfp4_matmul(copy(xp), copy(wp), out))
+
+
 def test_nothing_to_do():
     w = F.mxfp4_quantize(rows(10, 40, 1).cuda())
     assert F.mxfp4_matmul(torch.empty(0, 40, dtype=BF, device='cuda'), w).shape == (0, 10)
