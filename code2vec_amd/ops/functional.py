@@ -77,8 +77,9 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
     ctx (N,K); w_oi (2,H,K), gate then up, out-major like the tanh
     transform's shadow; activation one of GATE_ACTIVATIONS. Returns (y (N,H),
     kept): kept is what transform_gated_bwd needs if `save`, else None. It is
-    w_oi itself, which must not change in between: to form the projections again
-    takes no longer than to keep them in full. On the GPU all are bfloat16 (sums
+    w_oi itself, and no copy: to form the projections again takes no longer than
+    to keep them in full. A w_oi that was written to in between is refused by the
+    backward (a clone of kept is not concerned). On the GPU all are bfloat16 (sums
     and activation in fp32), any N, K and H; rows of ctx may be any stride apart."""
     if activation not in GATE_ACTIVATIONS:
         _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
@@ -93,7 +94,16 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
                                               GATE_ACTIVATIONS.index(activation))
     else:
         y = ref.transform_gated_fwd(ctx, w_oi, activation)
-    return y, w_oi if save else None
+    if not save:
+        return y, None
+    kept = w_oi.detach()        # the same memory, with the same count of writes
+    kept.writes = _writes(w_oi)
+    return y, kept
+
+
+def _writes(t) -> int:
+    """How often a tensor was written to, as far as torch counts that."""
+    return 0 if t.is_inference() else t._version
 
 
 def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
@@ -116,6 +126,8 @@ def transform_gated_bwd(ctx, w_io, kept, d_y, activation: str = 'silu',
         _refuse('the forward kept nothing: call it with save=True')
     if kept.shape != (2, d_y.shape[1], ctx.shape[1]):
         _refuse('the forward of this ctx kept something else')
+    if getattr(kept, 'writes', None) not in (None, _writes(kept)):
+        _refuse('w_oi has changed since the forward, which kept no copy of it')
     for t in (w_io, kept, d_y):
         if t.dtype != ctx.dtype or t.device != ctx.device:
             _refuse('ctx, w_io, kept and d_y must have one type and one device')

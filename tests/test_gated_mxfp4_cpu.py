@@ -92,6 +92,32 @@ def test_gated_weight_gradient_in_float32(dtype):
             F.transform_gated_bwd(x, w_io, kept, dy, dw_dtype=bad)
 
 
+def test_gated_weights_that_changed_in_between():
+    """The forward keeps no copy of the weights: the backward of others would be wrong."""
+    x, w_oi, w_io, dy = gated_inputs()
+    _, kept = F.transform_gated_fwd(x, w_oi, save=True)
+    own = kept.clone()
+    want = F.transform_gated_bwd(x, w_io, kept, dy)
+    w_oi[1].mul_(2.0)
+    with pytest.raises(ValueError, match='changed'):
+        F.transform_gated_bwd(x, w_io, kept, dy)
+    for a, b in zip(F.transform_gated_bwd(x, w_io, own, dy), want):
+        assert torch.equal(a, b)
+    # kept anew; two forwards keep apart; a read is no change
+    _, kept = F.transform_gated_fwd(x, w_oi, save=True)
+    w_oi.sum(), w_oi.cpu()
+    F.transform_gated_bwd(x, w_io, kept, dy)
+    w_oi.zero_()
+    F.transform_gated_bwd(x, w_io, F.transform_gated_fwd(x, w_oi, save=True)[1], dy)
+    with pytest.raises(ValueError, match='changed'):
+        F.transform_gated_bwd(x, w_io, kept, dy)
+    with torch.inference_mode():
+        v = w_oi.clone()
+        F.transform_gated_bwd(x, w_io, F.transform_gated_fwd(x, v, save=True)[1], dy)
+        F.transform_gated_bwd(x, w_io, F.transform_gated_fwd(x, w_oi, save=True)[1], dy)
+    F.transform_gated_bwd(x, w_io, F.transform_gated_fwd(x, v, save=True)[1], dy)
+
+
 def test_gated_refusals():
     x, w_oi, w_io, dy = gated_inputs()
     y, kept = F.transform_gated_fwd(x, w_oi, 'silu', save=True)
