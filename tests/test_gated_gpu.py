@@ -213,6 +213,42 @@ def test_dropout_mask_of_the_context(on_device):
     check_bwd(x, w_io, dy, 'gelu', d_ctx, d_w, keep=(mask, 0.75))
 
 
+@pytest.mark.parametrize('act', F.GATE_ACTIVATIONS)
+def test_each_activation_in_the_largest_tile(act):
+    """256 rows by 128 columns, which a last tile of 33 rows by 122 columns leaves ragged,
+    over a reduction that no step divides."""
+    x, w_oi, w_io, dy = make(20001, 390, 250, seed=6, scale=2.0)
+    y, kept, d_ctx, d_w = run(x, w_oi, w_io, dy, act)
+    check_fwd(x, w_oi, act, y, kept)
+    check_bwd(x, w_io, dy, act, d_ctx, d_w)
+
+
+@pytest.mark.parametrize('N,K,H', [(18000, 320, 256), (9003, 520, 500), (33001, 40, 120),
+                                   (50001, 64, 128), (14351, 136, 1440)])
+def test_sizes_of_the_largest_tile(N, K, H):
+    """Whole and ragged tiles, and reductions of one step, of two and of several."""
+    x, w_oi, w_io, dy = make(N, K, H, seed=N + K + H)
+    y, kept, d_ctx, d_w = run(x, w_oi, w_io, dy, 'silu')
+    check_fwd(x, w_oi, 'silu', y, kept)
+    check_bwd(x, w_io, dy, 'silu', d_ctx, d_w)
+
+
+@pytest.mark.parametrize('N,K,H', [(1, 24, 40), (300, 70, 1000), (5003, 192, 190),
+                                   (5003, 195, 190), (4099, 136, 520), (20011, 200, 190),
+                                   (20011, 198, 190)])
+def test_dropout_mask_in_every_tile(N, K, H):
+    """d_ctx in tiles of 32 by 32, 64 by 64 and 128 by 128, whole and ragged, with rows
+    of whole 16 bytes and others."""
+    x, w_oi, w_io, dy = make(N, K, H, seed=N + K + H)
+    seed = 2 ** 40 + N
+    y, kept, d_ctx, d_w = run(x, w_oi, w_io, dy, 'silu', keep_prob=0.75, seed=seed)
+    mask = R.dropout_keep_mask(seed, N * K, 0.75, 'cpu').reshape(N, K).double()
+    plain, same = F.transform_gated_bwd(x.cuda(), w_io.cuda(), kept, dy.cuda(), 'silu')
+    assert torch.equal(d_w, same)
+    assert torch.equal(d_ctx.cpu() == 0, (mask == 0) | (plain.cpu() == 0))
+    check_bwd(x, w_io, dy, 'silu', d_ctx, d_w, keep=(mask, 0.75))
+
+
 def test_nan_and_inf_stay_in_their_rows():
     x, w_oi, w_io, dy = make(100, 64, 64, seed=5)
     clean = run(x, w_oi, w_io, dy, 'silu')
