@@ -662,7 +662,8 @@ void check_mx(const torch::Tensor& codes, const torch::Tensor& scales, long K,
                     " must be on one GPU");
   TORCH_CHECK_VALUE(codes.scalar_type() == torch::kUInt8 &&
                     scales.scalar_type() == torch::kUInt8, name, " must be uint8");
-  TORCH_CHECK_VALUE(codes.dim() == 2 && scales.dim() == 2 &&
+  // (a K from -62 on would make no blocks, like none)
+  TORCH_CHECK_VALUE(K >= 0 && codes.dim() == 2 && scales.dim() == 2 &&
                     codes.size(0) == scales.size(0) && scales.size(1) == nb &&
                     codes.size(1) == 16 * nb, name, " does not hold rows of ", K);
   TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous(), name,

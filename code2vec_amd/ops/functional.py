@@ -153,7 +153,8 @@ def _check_mxfp4(q, name: str):
     if q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8:
         _refuse('%s must hold uint8 codes and scales', name)
     rows = q.scales.shape[0] if q.scales.dim() else 0
-    if q.codes.shape != (rows, 16 * blocks) or q.scales.shape != (rows, blocks):
+    if (q.k < 0 or q.codes.shape != (rows, 16 * blocks)
+            or q.scales.shape != (rows, blocks)):
         _refuse('%s does not hold rows of %d values: codes %s, scales %s', name, q.k,
                 tuple(q.codes.shape), tuple(q.scales.shape))
     if (not q.codes.is_contiguous() or not q.scales.is_contiguous()

@@ -196,6 +196,19 @@ def test_mxfp4_product_is_that_of_the_values():
     assert F.mxfp4_matmul(xb, wq).dtype == torch.bfloat16
 
 
+@pytest.mark.parametrize('k', [-1, -5, -62])
+def test_mxfp4_rows_of_no_length(k):
+    """Rows of fewer than no values, for which the number of blocks comes out as none."""
+    none = torch.empty(3, 0, dtype=torch.uint8)
+    bad = F.Mxfp4(none, none, k)
+    good = F.Mxfp4(none, none, 0)
+    assert F.mxfp4_matmul(good, good).shape == (3, 3)
+    for call in (lambda: F.mxfp4_dequantize(bad), lambda: F.mxfp4_matmul(bad, bad),
+                 lambda: F.mxfp4_matmul(torch.empty(3, 0, dtype=torch.bfloat16), bad)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_mxfp4_refusals():
     q = F.mxfp4_quantize(torch.randn(4, 40))
     x = torch.randn(3, 40).to(torch.bfloat16)

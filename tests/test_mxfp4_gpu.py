@@ -319,6 +319,16 @@ def test_offsets_beyond_32_bits():
         check_product(x[sl], w, y[sl], BF)
 
 
+@pytest.mark.parametrize('k', [-1, -5, -62])
+def test_rows_of_no_length(k):
+    none = torch.empty(3, 0, dtype=torch.uint8, device='cuda')
+    bad = F.Mxfp4(none, none, k)
+    for call in (lambda: F.mxfp4_dequantize(bad), lambda: F.mxfp4_matmul(bad, bad),
+                 lambda: F.mxfp4_matmul(torch.empty(3, 0, dtype=BF, device='cuda'), bad)):
+        with pytest.raises(ValueError, match='does not hold rows'):
+            call()
+
+
 def test_refusals():
     w = F.mxfp4_quantize(rows(10, 40, 1).cuda())
     x = rows(3, 40, 2, BF).cuda()
