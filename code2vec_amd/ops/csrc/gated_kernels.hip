@@ -7,11 +7,13 @@
 // The backward forms g and u again from x: to write and read them costs as
 // much, or loses precision. (204800 rows, K = H = 384, forward and backward: in
 // fp32 835 us, again 700; 14351 rows, 1440: 565 and 579; in bf16 670 and 476,
-// but with gradients off by 0.0030 where once rounded ones are by 0.0017 and
-// these by 0.0024.) bf16 operands, fp32 accumulation and activations. What is rounded to bf16 on the way are dg
-// and du, as operands of the two products that consume them; each such value
-// enters sums of 2H or N terms, so that a rounding of 2^-9 of a term stays one
-// of about 2^-9 of the result, which is itself rounded to bf16.
+// but with gradients off by 0.0030 of their norm where once rounded ones are by
+// 0.0017 and these by 0.0024.) bf16 operands, fp32 accumulation and activations.
+// What is rounded to bf16 on the way are dg and du, as operands of the two products
+// that consume them: each by at most 2^-8 of itself, so that a sum of 2H or N such
+// terms is off by at most 2^-8 of the sum of its terms' magnitudes, whatever of them
+// cancels. Their errors have either sign, and the 0.0024 is what they come to next to
+// the result's own rounding. dW may leave as it was summed, in fp32.
 
 #include <torch/extension.h>
 
@@ -22,8 +24,10 @@ namespace {
 
 enum Activation : int { SILU = 0, GELU = 1, SIGMOID = 2, TANH = 3, RELU = 4 };
 
-// The reciprocal and the exponential of the hardware are off by about one
-// step of fp32; their limits are right: 1 / (1 + exp(200)) is zero.
+// The hardware's reciprocal is off by about one step of fp32. Its exponential
+// takes g log2(e), whose rounding alone moves the result by about |g| steps: far
+// below bf16's 2^-8 wherever it counts. Their limits are right: 1 / (1 + exp(200))
+// is zero.
 DEVI float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-g));
 }
@@ -215,13 +219,15 @@ DEVI void put_plain(const BtArgs& p, ushort* to, long n, int h, const f32x4* a) 
   put<GT>(to, v, h, p.H);
 }
 
-// 204800 rows, K = H = 384: y 154 us (780 TFLOP/s), dg and du 217 us, dx 162 us;
-// 14351 rows of 1440: 135, 152 and 126 us (880, 780 and 950 TFLOP/s). The
-// matrix units are busy for 4/10 of the time (counted), which is 6/10 of what they
-// sustain without any loads, LDS for as long: a wave reads 12 KB for 32 products of
-// 16 cycles. Rounds of all blocks load, multiply and store in step, so that what
-// moves (314 MB for y, 630 for dg and du, at 5 TB/s) adds to that in part. The
-// epilogue of dg and du takes 18 vector instructions an element, 36 us in all.
+// 204800 rows, K = H = 384: y 141 us (860 TFLOP/s), dg and du 200 us, dx 158 us and
+// with the dropout mask 206; 14351 rows of 1440: 124, 131 and 116 us (960, 905 and
+// 1030 TFLOP/s). Counted at 204800 rows (profiles/gated_mxfp4_counters.csv), of the
+// cycles in which a CU has waves: the matrix units work in 38% for y, 26% for dg
+// and du and 32% for dx, LDS reads in 14, 10 and 16%, without bank conflicts. None of
+// them is full: what is left are waits, because rounds of all blocks load, multiply
+// and store in step, so that what moves (314 MB for y, 630 for dg and du, at 5
+// TB/s) adds to the products in part. The epilogue of dg and du takes 18 vector
+// instructions an element; the mask is a hash of 64 bits for each element of dx.
 template <int EPI, int ACT, int WR, int WC, int XT, int GT, int BK,
           int STAGES>
 __launch_bounds__(WR * WC * 64, 2)
@@ -491,8 +497,8 @@ __global__ void k_rows_gemm(BtArgs p) {
 // one after the other: a block's four waves share 16 columns (of gate and up;
 // 32 of a plain product) and cut the reduction, step by step in turn; their
 // sums are added in order in LDS. Operands go from memory to registers, two
-// steps ahead. (200 rows, K = H = 384: 4.6 us, where the tiles of 64 by 32 take
-// 4.7 and an empty launch 2.)
+// steps ahead. (200 rows, K = H = 384: 4.2 us; side by side 4.6, where the
+// tiles of 64 by 32 took 4.7 and an empty launch 2.)
 template <int EPI, int ACT, int XT>
 __launch_bounds__(256)
 __global__ void k_rows_skinny(BtArgs p) {
@@ -583,9 +589,9 @@ __global__ void k_rows_skinny(BtArgs p) {
 // neighbouring rows, whose 32-byte units the exclusive-or below spreads over
 // all banks. N is split over blocks; the parts are added in order by
 // k_dw_reduce, so that a result never depends on timing.
-// 204800 rows, K = H = 384: 170 us (710 TFLOP/s, 472 MB read and 66 written),
-// the parts' sum 12 us; 14351 rows of 1440: 158 us (750 TFLOP/s) and 11. Bound as
-// the products above. Reading the next step's operands ahead needs registers that
+// 204800 rows, K = H = 384: 155 us (780 TFLOP/s, 472 MB read and 66 written),
+// the parts' sum 12 us; 14351 rows of 1440: 144 us (830 TFLOP/s) and 11. Bound as
+// the products above: matrix units 33% of the cycles, LDS reads 13%. Reading the next step's operands ahead needs registers that
 // the sums take (272 us with spills; with sums of 192 by 128, 211).
 // ---------------------------------------------------------------------------
 
@@ -867,7 +873,8 @@ double launch_us(double blocks, double slots, double steps, double alone,
 // Tiles from 256 rows by 128 columns of gate and up down to 16 by 16: large
 // ones read least, small ones fill the chip. The rates are fitted to both
 // products at 1..204800 rows and widths of 96..1440; what they choose is the
-// best or within a tenth of it at six sizes of seven. The gated product, in us:
+// best or within a tenth of it at six sizes of seven. The gated product, in us (20
+// calls of each; in a longer run the last row's first is 141, the one above it 124):
 //   rows  width   256x128   128x64   64x32   32x16
 //    200    384      13.1      6.7     4.7     4.6
 //   1024    768      22.9     11.3     8.7    19.5
@@ -904,7 +911,7 @@ void rows_gemm(const BtArgs& a) {
 // more than fills the chip costs a whole round, and every part costs the
 // writing and reading of its sums. Fitted like the rates of rows_gemm; what is
 // chosen is the best of these, or within 13% of it, at ten sizes. In us, each
-// tile with its best number of parts, their sum included:
+// tile with its best number of parts, their sum included (20 calls of each, as above):
 //   rows  K to H       256x128   128x128   64x64
 //    512  192 to 192      11.8       9.7     8.3
 //   2000 1000 to 1000     30.0      27.0    29.5

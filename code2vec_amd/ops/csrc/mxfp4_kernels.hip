@@ -77,8 +77,8 @@ DEVI bf16x8 decode8(u32 codes, float scale) {
 // and saturates to 6); it is taken from the bits, whose order as integers is
 // that of the magnitudes, with infinities and NaN on top. The conversion
 // instruction rounds to nearest, ties to the even code. One pass, bound by
-// memory: 261246 rows of 384 float32 (401 MB read, 53 written) in 96 us, 4.7
-// TB/s; back to bf16 (53 read, 201 written) in 44 us, 5.7 TB/s.
+// memory: 261246 rows of 384 float32 (401 MB read, 53 written) in 99 us, 4.6
+// TB/s; back to bf16 (53 read, 201 written) in 46 us, 5.6 TB/s.
 // ---------------------------------------------------------------------------
 
 template <bool F32>
@@ -199,9 +199,10 @@ __global__ void k_mxfp4_dequantize(const u32* __restrict__ codes,
 // Lane (i, q) holds block 4s + q of its row in step s of 128 values: for x in
 // bf16 sub-step j multiplies values 8j..8j+7 of that block.
 //
-// One row by 261246 of 384: 12.0 us, bound by the reading of w (53 MB, 4.4 TB/s,
+// One row by 261246 of 384: 13.3 us, bound by the reading of w (53 MB, 4.0 TB/s,
 // where bf16 weights would be 201 MB). 37 rows by 50001 of 201, y in float32:
-// 9.0 us, bound by y's broken lines (7.4 MB) and by latency.
+// 9.7 us, bound by latency, in blocks that live for one pass, and by y's broken lines
+// (7.4 MB).
 // ---------------------------------------------------------------------------
 
 struct MxArgs {
@@ -430,9 +431,11 @@ __global__ void k_mxfp4_rows(MxArgs p) {
 // pass but at the table's ends, because rows of x behind the last one repeat
 // it, and store the same again.
 //
-// 261246 columns, K = 384, y in bf16: 1024 rows of bf16 207 us (535 MB written,
-// 990 TFLOP/s; bound by the decoding of w, which every wave does for its 32 rows,
-// next to the products), 4096 rows in 4 bits 516 us (2.1 GB, 4.1 TB/s: writing).
+// 261246 columns, K = 384, y in bf16: 1024 rows of bf16 206 us (535 MB written,
+// 1000 TFLOP/s; bound by the decoding of w, which every wave does for its 32 rows,
+// next to the products: matrix units work in 45% of the cycles, and 3.4 other vector
+// instructions go with each of theirs), 4096 rows in 4 bits 516 us (2.1 GB, 4.1
+// TB/s: writing).
 template <bool X4, bool OUT32, int R>
 struct Stream {
   static constexpr int XT = X4 ? 4 : R > 4 ? 1 : 2;   // 16-row tiles of x a wave

@@ -56,6 +56,9 @@ def main():
     timeit('gated transform fwd', lambda: F.transform_gated_fwd(ctx, gw_oi))
     timeit('gated transform bwd',
            lambda: F.transform_gated_bwd(ctx, gw_io, gw_oi, d_y))
+    timeit('gated transform bwd, as in training',
+           lambda: F.transform_gated_bwd(ctx, gw_io, gw_oi, d_y, keep_prob=0.75, seed=7,
+                                         dw_dtype=torch.float32))
 
     timeit('logits hipBLASLt', lambda: code @ shadow.t())
     timeit('logits our gemm_bt', lambda: ext.gemm_bt_bf16(code, shadow))
