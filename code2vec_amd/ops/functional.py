@@ -79,8 +79,9 @@ def transform_gated_fwd(ctx, w_oi, activation: str = 'silu', save: bool = False
     kept): kept is what transform_gated_bwd needs if `save`, else None. It is
     w_oi itself, and no copy: to form the projections again takes no longer than
     to keep them in full. If w_oi, or a buffer that it is a part of, was written
-    to in between, the backward refuses it (a clone of kept is not concerned). On the GPU all are bfloat16 (sums
-    and activation in fp32), any N, K and H; rows of ctx may be any stride apart."""
+    to in between, the backward refuses it (a clone of kept is not concerned). On
+    the GPU all are bfloat16 (sums and activation in fp32), any N, K and H; rows of
+    ctx may be any stride apart."""
     if activation not in GATE_ACTIVATIONS:
         _refuse('activation must be one of %s, not %r', GATE_ACTIVATIONS, activation)
     if (ctx.dim() != 2 or w_oi.dim() != 3 or w_oi.shape[0] != 2
